@@ -453,6 +453,105 @@ Q3_API int q3_batch_logits(q3_batch* b, uint32_t seq, uint16_t* out);
 Q3_API int q3_batch_info(q3_batch* b, uint32_t seq, size_t* position, size_t* free_pages);
 
 /* ------------------------------------------------------------------------
+ * Bounded paged KV cache (op level; no counterpart in the reference, whose
+ * cache grows until the context is full: src/lib/kv_cache/kv_cache.hpp:6-29).
+ *
+ * One layer's cache of `rows` sequences.  K and V live in the library's pages
+ * [num_pages, kv_heads, 64, 128]; sequence r keeps its slots 0 .. len - 1 in
+ * the pages page_tables[r * table_stride + slot / 64].  A slot is not a token
+ * position: keys are stored with their rotary position applied, attention does
+ * not depend on the order of the slots, and an eviction moves slots.  Per
+ * sequence, kv head and slot the cache keeps, at
+ * [(r * kv_heads + h) * slot_stride + slot], the attention the slot has
+ * received so far (weights, fp32) and the token position it holds (positions).
+ *
+ * Per decoded token:  q3_cache_append  (q/k RMSNorm + RoPE at the position, K
+ * and V into slot len), q3_cache_attention (over slots 0 .. len, weights
+ * accumulated) and, whenever a sequence should shrink, q3_cache_evict.
+ *
+ * All calls are asynchronous on `stream`, launch nothing but kernels and can be
+ * captured into CUDA graphs: lengths, slots, positions and page tables are read
+ * from device memory.  The caller owns every buffer, the handle only describes
+ * them.  Values in device memory that are out of range
+ * (a page outside the pool, a length or slot past max_len, a position past the
+ * RoPE tables) are never followed: the row is skipped (attention: its output is
+ * NaN) and q3_cache_sync reports Q3_ERR_DEVICE.
+ * ---------------------------------------------------------------------- */
+typedef struct q3_cache q3_cache;
+
+typedef struct q3_cache_desc {
+    uint16_t* k_pages_dev; /* [num_pages, kv_heads, page_size, head_dim] */
+    uint16_t* v_pages_dev;
+    size_t num_pages;
+    const int32_t* page_tables_dev; /* row r: ceil(max_len / 64) entries at r * table_stride */
+    size_t table_stride;
+    float* weights_dev;     /* may be NULL: no accumulated weights, no eviction */
+    int32_t* positions_dev; /* NULL exactly when weights_dev is */
+    size_t slot_stride;     /* >= max_len */
+    size_t rows;            /* sequences, 1 .. 4096 */
+    size_t max_len;         /* slots a sequence may hold, 1 .. 2^20 */
+    size_t kv_heads;
+    size_t head_dim;  /* 128 */
+    size_t page_size; /* 64 */
+    uint32_t* error_dev; /* one word, 0 at first: the first error that a kernel of this cache met */
+} q3_cache_desc;
+
+/* The handle works on `device`, whichever device is current when it is used.
+ * Creating one touches no GPU. */
+Q3_API int q3_cache_create(const q3_cache_desc* desc, int device, q3_cache** out);
+Q3_API int q3_cache_destroy(q3_cache* c);
+
+/* Blocks until `stream` has finished, then reports (and clears) the error word:
+ * Q3_ERR_DEVICE with its cause if a kernel recorded one. */
+Q3_API int q3_cache_sync(q3_cache* c, void* stream);
+
+/* Writes n new tokens into the cache.  Row i holds q_heads query heads, kv_heads
+ * key heads and kv_heads value heads of 128 (at q + i * q_stride, ...; strides
+ * in elements, multiples of 8: the three may be slices of one QKV row).  Heads
+ * are normalised and rotated as q3_qk_norm_rope does at token_pos[i]; queries go
+ * to q_out + i * q_out_stride (q_out may be q with its stride), keys and values
+ * to slot slots[i] of sequence row_seq[i] (row_seq NULL: sequence i, n <= rows),
+ * whose weights become 0 and positions token_pos[i].  lens_out (may be NULL, may
+ * be slots): lens_out[i] = slots[i] + 1.  A row with slots[i] = -1 is skipped.
+ * Rows of one call have different (sequence, slot) pairs.  The RoPE tables
+ * [max_pos, 64] cover positions 0 .. max_pos - 1. */
+Q3_API int q3_cache_append(q3_cache* c, const uint16_t* q_dev, size_t q_stride, const uint16_t* k_dev, size_t k_stride,
+                           const uint16_t* v_dev, size_t v_stride, const uint16_t* q_norm_dev,
+                           const uint16_t* k_norm_dev, const float* cos_dev, const float* sin_dev, size_t max_pos,
+                           const int32_t* token_pos_dev, const int32_t* slots_dev, const int32_t* row_seq_dev,
+                           size_t n, size_t q_heads, uint16_t* q_out_dev, size_t q_out_stride, int32_t* lens_out_dev,
+                           float eps, void* stream);
+
+/* Attention of one query token per sequence over its slots 0 .. lens[r] - 1:
+ * out = softmax(q K^T / sqrt(128)) V per query head with the GQA map
+ * kv = qh / (q_heads / kv_heads), fp32 softmax, BF16 out.  q_heads is kv_heads
+ * times 1 .. 16.  With accumulate != 0 every slot's softmax probabilities,
+ * summed over the query heads of its kv head, are added to its weight.  A
+ * sequence of length 0 gets zeros and keeps its weights.  out may be q (with
+ * its stride).  Strides in elements, multiples of 8.  The workspace (16-byte
+ * aligned, q3_cache_attention_workspace_bytes) belongs to the call until it has
+ * finished on the GPU; calls on unordered streams need one each. */
+Q3_API size_t q3_cache_attention_workspace_bytes(const q3_cache* c, size_t q_heads, int accumulate);
+Q3_API int q3_cache_attention(q3_cache* c, const uint16_t* q_dev, size_t q_stride, const int32_t* lens_dev,
+                              uint16_t* out_dev, size_t out_stride, size_t q_heads, int accumulate,
+                              void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* Shrinks every sequence longer than `keep` to keep slots, per kv head: slots
+ * whose position is >= next_pos[r] - recent are kept first, then those with the
+ * largest accumulated weight (NaN counts as the smallest), the lower slot first
+ * among equals.  Kept slots behind `keep` move into the evicted slots before it,
+ * both in ascending order (K, V, weights, positions); nothing else moves.
+ * weights_out / positions_out (both or neither NULL; the layout of weights /
+ * positions): receive slots 0 .. min(len, keep) - 1 and leave the cache's own
+ * arrays, which they must not overlap, as they were; NULL: in place.  lens_out[r] = min(lens[r], keep);
+ * lens_out may be lens.  The pages of a sequence that shrinks must not be shared
+ * with another.  Pages ceil(keep / 64) and up are free afterwards. */
+Q3_API size_t q3_cache_evict_workspace_bytes(const q3_cache* c, size_t keep);
+Q3_API int q3_cache_evict(q3_cache* c, const int32_t* lens_dev, const int32_t* next_pos_dev, size_t keep,
+                          size_t recent, float* weights_out_dev, int32_t* positions_out_dev, int32_t* lens_out_dev,
+                          void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Tokenizer and text generation (host code): tokenizer::Tokenizer
  * (src/lib/tokenizer/tokenizer.hpp:35-66, tokenizer.cpp:205-265) and
  * Generator::generate on text (src/lib/inference/generator.cpp:37-63).

@@ -99,6 +99,15 @@ SIGNATURES = {
     "q3_batch_tokens": (C.c_int, [_vp, C.c_uint32, _u32p, _sz, _szp]),
     "q3_batch_logits": (C.c_int, [_vp, C.c_uint32, _u16p]),
     "q3_batch_info": (C.c_int, [_vp, C.c_uint32, _szp, _szp]),
+    "q3_cache_create": (C.c_int, [_vp, C.c_int, C.POINTER(C.c_void_p)]),
+    "q3_cache_destroy": (C.c_int, [_vp]),
+    "q3_cache_sync": (C.c_int, [_vp, _vp]),
+    "q3_cache_append": (C.c_int, [_vp, _u16p, _sz, _u16p, _sz, _u16p, _sz, _u16p, _u16p, _vp, _vp, _sz, _i32p, _i32p,
+                                  _i32p, _sz, _sz, _u16p, _sz, _i32p, C.c_float, _vp]),
+    "q3_cache_attention_workspace_bytes": (_sz, [_vp, _sz, C.c_int]),
+    "q3_cache_attention": (C.c_int, [_vp, _u16p, _sz, _i32p, _u16p, _sz, _sz, C.c_int, _vp, _sz, _vp]),
+    "q3_cache_evict_workspace_bytes": (_sz, [_vp, _sz]),
+    "q3_cache_evict": (C.c_int, [_vp, _i32p, _i32p, _sz, _sz, _vp, _vp, _i32p, _vp, _sz, _vp]),
 }
 
 
@@ -138,6 +147,16 @@ class ModelConfig(C.Structure):
                 ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("vocab", C.c_uint32), ("tied", C.c_uint32),
                 ("eps", C.c_float), ("theta", C.c_float), ("capacity", C.c_uint32), ("eos", C.c_uint32),
                 ("weight_format", C.c_uint32)]
+
+
+class CacheDesc(C.Structure):
+    """q3_cache_desc (include/q3_sm100a.h)."""
+
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("num_pages", C.c_size_t),
+                ("page_tables", C.c_void_p), ("table_stride", C.c_size_t), ("weights", C.c_void_p),
+                ("positions", C.c_void_p), ("slot_stride", C.c_size_t), ("rows", C.c_size_t),
+                ("max_len", C.c_size_t), ("kv_heads", C.c_size_t), ("head_dim", C.c_size_t),
+                ("page_size", C.c_size_t), ("error", C.c_void_p)]
 
 
 WEIGHT_FORMATS = {"bf16": 0, "fp8": 1, "nvfp4": 2}  # Q3_WEIGHTS_BF16, Q3_WEIGHTS_FP8_E4M3, Q3_WEIGHTS_NVFP4

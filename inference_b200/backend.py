@@ -150,6 +150,96 @@ class B200Backend:
         check(lib().q3_qk_norm_rope(_p(query), _p(key), _p(q_norm), _p(k_norm), _p(cache.cosine), _p(cache.sine),
                                     query.shape[0], key.shape[0], query.shape[1], token_pos, eps, self._stream()))
 
+    # ---- bounded paged KV cache (cache.py, q3_cache_*): no counterpart in backend.hpp
+
+    def _rows(self, name: str, t, n: int, heads: int | None = None):
+        """t is a bf16 [n, heads, 128] tensor on this device whose rows are contiguous; returns its row stride."""
+        torch = _torch()
+        if t.dtype != torch.bfloat16 or t.dim() != 3 or t.device != self.device:
+            raise ValueError(f"{name} must be a bf16 [rows, heads, 128] tensor on {self.device}")
+        if t.shape[0] != n or t.shape[2] != 128 or (heads is not None and t.shape[1] != heads):
+            raise ValueError(f"{name}: shape {tuple(t.shape)} does not fit")
+        stride = t.stride()
+        if stride[2] != 1 or (stride[1] != 128 and t.shape[1] > 1):
+            raise ValueError(f"{name}: the heads of a row must be contiguous")
+        return stride[0] if n > 1 else 128 * t.shape[1]
+
+    def _ints(self, name: str, t, n: int) -> int:
+        if t.dtype != _torch().int32 or t.device != self.device or tuple(t.shape) != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor of {n} on {self.device}")
+        return t.data_ptr()
+
+    def _scratch(self, need: int):
+        # from torch's stream-ordered allocator at every call: calls on different streams and
+        # captured graphs never share one
+        torch = _torch()
+        return torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
+
+    def _own(self, cache):
+        if cache.device != self.device:
+            raise ValueError(f"the cache is on {cache.device}, this backend on {self.device}")
+
+    def cache_append(self, cache, query, key, value, q_norm, k_norm, rope: RopeCache, token_pos, slots, query_out,
+                     epsilon: float, lens_out=None, row_seq=None):
+        """New tokens into `cache` (q3_cache_append): row i of query / key / value (bf16 [n, heads, 128], rows may
+        be strided) is normalised and rotated as qk_norm_rope does at token_pos[i]; the query goes to query_out (may
+        be query), key and value to slot slots[i] of sequence row_seq[i] (None: sequence i).  slots[i] = -1 skips
+        the row.  lens_out[i] = slots[i] + 1 (may be slots)."""
+        self._own(cache)
+        torch = _torch()
+        n, qh = query.shape[0], query.shape[1]
+        qs = self._rows("query", query, n)
+        ks = self._rows("key", key, n, cache.kv_heads)
+        vs = self._rows("value", value, n, cache.kv_heads)
+        os_ = self._rows("query_out", query_out, n, qh)
+        for t in (q_norm, k_norm):
+            if t.dtype != torch.bfloat16 or t.numel() != 128 or not t.is_contiguous() or t.device != self.device:
+                raise ValueError("q_norm and k_norm must be contiguous bf16 tensors of 128")
+        for t in (rope.cosine, rope.sine):
+            if (t.dtype != torch.float32 or t.shape != rope.cosine.shape or t.shape[1] != 64 or not t.is_contiguous()
+                    or t.device != self.device):
+                raise ValueError("RoPE tables must be contiguous fp32 [positions, 64]")
+        check(lib().q3_cache_append(
+            cache.h, _p(query), qs, _p(key), ks, _p(value), vs, _p(q_norm), _p(k_norm), _p(rope.cosine),
+            _p(rope.sine), rope.cosine.shape[0], self._ints("token_pos", token_pos, n), self._ints("slots", slots, n),
+            None if row_seq is None else self._ints("row_seq", row_seq, n), n, qh, _p(query_out), os_,
+            None if lens_out is None else self._ints("lens_out", lens_out, n), epsilon, self._stream()))
+
+    def cache_attention(self, cache, query, lens, output, accumulate: bool = True):
+        """output[r] = attention of query[r] (bf16 [rows, q_heads, 128], rows may be strided) over slots
+        0 .. lens[r] - 1 of sequence r (q3_cache_attention); accumulate adds each slot's probabilities, summed over
+        the query heads of its kv head, to cache.weights.  output may be query."""
+        self._own(cache)
+        L = lib()
+        qh = query.shape[1]
+        qs = self._rows("query", query, cache.rows)
+        os_ = self._rows("output", output, cache.rows, qh)
+        need = L.q3_cache_attention_workspace_bytes(cache.h, qh, accumulate)
+        ws = self._scratch(need)
+        check(L.q3_cache_attention(cache.h, _p(query), qs, self._ints("lens", lens, cache.rows), _p(output), os_, qh,
+                                   accumulate, _p(ws), ws.numel(), self._stream()))
+
+    def cache_evict(self, cache, lens, next_pos, keep: int, recent: int, lens_out, weights_out=None,
+                    positions_out=None):
+        """Shrinks every sequence longer than `keep` to `keep` slots per kv head (q3_cache_evict): slots at positions
+        >= next_pos[r] - recent first, then the largest weights, the lower slot among equals.  In place, or weights
+        and positions to weights_out and positions_out (laid out as the cache's).  lens_out[r] = min(lens[r], keep)
+        (may be lens)."""
+        self._own(cache)
+        L = lib()
+        for t, like in ((weights_out, cache.weights), (positions_out, cache.positions)):
+            if t is not None and (like is None or t.dtype != like.dtype or t.shape != like.shape or
+                                  t.stride() != like.stride() or t.device != self.device):
+                raise ValueError("weights_out and positions_out must be laid out as the cache's")
+        if keep < 1 or recent < 0:
+            raise ValueError("cache_evict: keep must be at least 1 and recent at least 0")
+        ws = self._scratch(L.q3_cache_evict_workspace_bytes(cache.h, keep))
+        check(L.q3_cache_evict(cache.h, self._ints("lens", lens, cache.rows),
+                               self._ints("next_pos", next_pos, cache.rows), keep, recent,
+                               None if weights_out is None else _p(weights_out),
+                               None if positions_out is None else _p(positions_out),
+                               self._ints("lens_out", lens_out, cache.rows), _p(ws), ws.numel(), self._stream()))
+
     # backend.hpp:35 -- synchronises to return the id, as the reference does
     def argmax(self, logits) -> int:
         torch = _torch()

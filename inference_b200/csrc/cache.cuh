@@ -1,0 +1,75 @@
+// cache.cuh -- the bounded paged KV cache: device view and launchers of its
+// operators (append, attention with accumulated weights, eviction).
+#pragma once
+
+#include "kernels.cuh"
+
+namespace q3 {
+
+constexpr int kCachePage = 64;  // slots per page
+constexpr int kCacheHd = 128;   // head dimension
+
+// One layer's cache as the kernels see it (q3_cache_desc).  Slot s of sequence r,
+// kv head h: K/V row ((page_table(r)[s / 64] * kv_heads + h) * 64 + s % 64) * 128,
+// weights and positions at (r * kv_heads + h) * slot_stride + s.
+struct CacheView {
+    bf16 *k, *v;
+    int num_pages;
+    const int32_t* tables;
+    long long table_stride;
+    float* weights;
+    int32_t* positions;
+    long long slot_stride;
+    int rows, max_len, kv_heads;
+    uint32_t* err;
+};
+
+__host__ __device__ inline size_t cache_slot_index(const CacheView& c, int row, int head) {
+    return (static_cast<size_t>(row) * c.kv_heads + head) * c.slot_stride;
+}
+__device__ __forceinline__ size_t cache_kv_offset(const CacheView& c, int page, int head, int slot) {
+    return ((static_cast<size_t>(page) * c.kv_heads + head) * kCachePage + slot % kCachePage) * kCacheHd;
+}
+
+struct CacheAppendArgs {
+    CacheView c;
+    const bf16 *q, *k, *v;
+    long long q_stride, k_stride, v_stride;
+    const bf16 *q_norm, *k_norm;
+    const float *rope_cos, *rope_sin;
+    int max_pos;
+    const int32_t *token_pos, *slots, *row_seq;
+    int n, q_heads;
+    bf16* q_out;
+    long long q_out_stride;
+    int32_t* lens_out;
+    float eps;
+};
+cudaError_t launch_cache_append(const CacheAppendArgs& a, cudaStream_t s);
+
+struct CacheAttnArgs {
+    CacheView c;
+    const bf16* q;
+    long long q_stride;
+    const int32_t* lens;
+    bf16* out;
+    long long out_stride;
+    int q_heads, accumulate;
+    void* ws;
+};
+size_t cache_attention_ws_bytes(const CacheView& c, int q_heads, int accumulate, int sms);
+cudaError_t launch_cache_attention(const CacheAttnArgs& a, int sms, cudaStream_t s);
+
+struct CacheEvictArgs {
+    CacheView c;
+    const int32_t *lens, *next_pos;
+    int keep, recent;
+    float* weights_out;      // null: in place
+    int32_t* positions_out;  // null: in place
+    int32_t* lens_out;
+    void* ws;
+};
+size_t cache_evict_ws_bytes(const CacheView& c, int keep);
+cudaError_t launch_cache_evict(const CacheEvictArgs& a, cudaStream_t s);
+
+}  // namespace q3

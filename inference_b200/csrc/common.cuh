@@ -26,6 +26,10 @@ enum DeviceError : uint32_t {
     DEV_BAD_TOKEN = 3,
     DEV_BAD_POSITION = 4,
     DEV_GRID_TIMEOUT = 5,
+    DEV_BAD_PAGE = 6,
+    DEV_BAD_LENGTH = 7,
+    DEV_BAD_SLOT = 8,
+    DEV_BAD_SEQUENCE = 9,
 };
 
 // Upper bound on mbarrier polls before a kernel gives up (each try_wait

@@ -1,0 +1,530 @@
+"""The bounded paged KV cache on the GPU: append, attention with accumulated
+weights and eviction, each against a plain form in 64 bits (cache_util.py), and
+a decode loop of the three together."""
+import math
+
+import numpy as np
+import pytest
+
+import cache_util as cu
+from cache_util import HD, PAGE, Setup, close, ints
+
+pytestmark = pytest.mark.gpu
+EPS = 1e-6
+
+
+@pytest.fixture(scope="module")
+def be():
+    from inference_b200 import B200Backend
+
+    return B200Backend(0)
+
+
+def bits(t):
+    import torch
+
+    return t.view(torch.int16 if t.dtype == torch.bfloat16 else torch.int32)
+
+
+def same(a, b):
+    import torch
+
+    return torch.equal(bits(a), bits(b))
+
+
+def check_attention(be, s, cache, q, lens, accumulate=True, out=None):
+    import torch
+
+    want, tol, dw, dw_tol = cu.attention(s, q, lens)
+    before = s.w.clone() if s.w is not None else None
+    out = torch.full_like(q, 7.0) if out is None else out
+    be.cache_attention(cache, q, ints(lens), out, accumulate=accumulate)
+    cache.sync()
+    close(out, want, tol, "out")
+    if accumulate:
+        full = before.double() + dw
+        # one more rounding: the addition to the weight
+        close(s.w, full, dw_tol + full.abs() * 2.0 ** -23, "weights")
+        for r, n in enumerate(lens):  # slots behind the length keep their weights bit for bit
+            assert same(s.w[r, :, n:], before[r, :, n:])
+    elif before is not None:
+        assert same(s.w, before)
+    return out
+
+
+LENS = [[1], [0], [2, 0, 1, 64, 63, 65, 128, 127, 129, 15, 16, 17, 33, 300], [1000], [4095], [20000, 3, 700]]
+
+
+@pytest.mark.parametrize("qh,kvh", [(8, 8), (16, 8), (32, 8), (64, 8), (8, 1), (16, 1), (12, 4), (5, 1), (22, 2), (7, 7)])
+@pytest.mark.parametrize("lens", LENS, ids=lambda v: "x".join(map(str, v)))
+def test_attention(be, qh, kvh, lens):
+    """Every head-group size and lengths around page and fragment borders, on a shuffled pool whose unused slots hold NaN
+    and infinity (they must not reach any output)."""
+    s = Setup(len(lens), kvh, max(max(lens), 1), seed=qh * 100 + len(lens))
+    s.behind(s.k, lens, math.nan)
+    s.behind(s.v, lens, math.inf if qh % 2 else math.nan)
+    q = s.randn(len(lens), qh, HD)
+    with s.cache() as cache:
+        check_attention(be, s, cache, q, lens)
+
+
+@pytest.mark.parametrize("accumulate", [True, False])
+def test_attention_many_rows(be, accumulate):
+    rng = np.random.default_rng(5)
+    lens = [int(x) for x in rng.integers(0, 700, 300)]
+    s = Setup(300, 2, 700, seed=1)
+    q = s.randn(300, 8, HD)
+    with s.cache() as cache:
+        check_attention(be, s, cache, q, lens, accumulate)
+
+
+def test_attention_most_rows(be):
+    """The largest number of sequences, most of them idle."""
+    lens = [0] * 4096
+    lens[0], lens[1000], lens[4095] = 70, 1, 130
+    s = Setup(4096, 1, 130, seed=2)
+    q = s.randn(4096, 2, HD)
+    with s.cache() as cache:
+        check_attention(be, s, cache, q, lens)
+
+
+def test_attention_strided_rows_padded_slots_and_alias(be):
+    """Queries as a slice of a wider row, weights with padding behind the slots, the output over the query; max_len below
+    what the buffers cover."""
+    import torch
+
+    lens = [100, 1, 77]
+    s = Setup(3, 4, 130, seed=3, slot_stride=150)
+    wide = s.randn(3, 8 + 4 + 4, HD)
+    q = wide[:, :8]
+    rest = wide[:, 8:].clone()
+    want = q.clone()
+    with s.cache(max_len=101) as cache:
+        first = check_attention(be, s, cache, want, lens, False)
+        be.cache_attention(cache, q, ints(lens), q, accumulate=False)
+        cache.sync()
+        assert same(q.contiguous(), first) and same(wide[:, 8:].contiguous(), rest)
+        strided = torch.zeros(3, 11, HD, dtype=torch.bfloat16, device="cuda")
+        check_attention(be, s, cache, want, lens, True, out=strided[:, 2:10])
+        assert not strided[:, :2].any() and not strided[:, 10:].any()
+
+
+def test_attention_of_sharp_and_extreme_scores(be):
+    """Scores far apart (one slot takes all), equal everywhere, and so large that exp overflows without the maximum."""
+    s = Setup(3, 1, 200, seed=4)
+    lens = [200, 200, 190]
+    q = s.randn(3, 4, HD)
+    q[0] *= 40.0
+    q[1] = 0.0
+    s.k[s.tables[2, 1].long(), 0, 5] = q[2, 1] * 30.0
+    with s.cache() as cache:
+        check_attention(be, s, cache, q, lens)
+
+
+def test_attention_of_nan_and_infinity_in_live_slots(be):
+    """What lives in a used slot counts, as in the formula: NaN in a key or value reaches its own sequence and head and no
+    other; an infinite value makes its dimension infinite or NaN (the probabilities are multiplied in two parts); a key
+    that makes a score -inf drops its slot."""
+    import torch
+
+    lens = [70, 70, 70, 70, 10]
+    s = Setup(5, 2, 70, seed=6)
+    q = s.randn(5, 4, HD).abs() + 0.1
+    s.k[s.tables[0, 1].long(), 0, 3, 7] = math.nan
+    s.v[s.tables[1, 0].long(), 1, 9, 100] = math.nan
+    s.v[s.tables[2, 0].long(), 0, 9, 4] = math.inf
+    s.k[s.tables[3, 0].long(), 1, 20, 0] = -math.inf
+    before = s.w.clone()
+    out = torch.empty_like(q)
+    with s.cache() as cache:
+        be.cache_attention(cache, q, ints(lens), out)
+        cache.sync()
+    want, tol, dw, _ = cu.attention(s, q, lens)
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(out), fine)
+    assert bool(torch.isnan(out)[torch.isnan(want)].all())
+    close(out[fine], want[fine], tol[fine])
+    assert torch.equal(torch.isnan(s.w), torch.isnan(before.double() + dw))
+    assert float(s.w[3, 1, 20]) == float(before[3, 1, 20])
+
+
+@pytest.mark.parametrize("bad", ["page_high", "page_negative", "length_high", "length_negative"])
+def test_attention_refuses_bad_device_values(be, bad):
+    """A page outside the pool or a length outside the cache poisons its own row (NaN) and no other, leaves that row's
+    weights, and is reported once."""
+    import torch
+
+    from inference_b200 import Q3Error
+
+    lens = [100, 150, 64]
+    s = Setup(3, 2, 150, seed=7)
+    q = s.randn(3, 4, HD)
+    want, tol, dw, dw_tol = cu.attention(s, q, lens)
+    before = s.w.clone()
+    given = list(lens)
+    if bad == "page_high":
+        s.tables[1, 2] = s.k.shape[0]
+    elif bad == "page_negative":
+        s.tables[1, 0] = -1
+    else:
+        given[1] = 151 if bad == "length_high" else -5
+    out = torch.zeros_like(q)
+    with s.cache() as cache:
+        be.cache_attention(cache, q, ints(given), out)
+        with pytest.raises(Q3Error) as e:
+            cache.sync()
+        assert e.value.status == 5 and ("page" if bad.startswith("page") else "length") in str(e.value)
+        cache.sync()  # reported and cleared
+    assert torch.isnan(out[1]).all()
+    close(out[[0, 2]], want[[0, 2]], tol[[0, 2]])
+    full = before.double() + dw
+    close(s.w[[0, 2]], full[[0, 2]], (dw_tol + full.abs() * 2.0 ** -23)[[0, 2]])
+    assert same(s.w[1], before[1])
+
+
+def test_attention_is_deterministic(be):
+    import torch
+
+    lens = [5000, 17, 900, 64]
+    s = Setup(4, 8, 5000, seed=8)
+    q = s.randn(4, 32, HD)
+    start = s.w.clone()
+    got = []
+    with s.cache() as cache:
+        for _ in range(3):
+            s.w.copy_(start)
+            out = torch.empty_like(q)
+            be.cache_attention(cache, q, ints(lens), out)
+            cache.sync()
+            got.append((out, s.w.clone()))
+    assert all(same(a, got[0][0]) and same(b, got[0][1]) for a, b in got)
+
+
+def tables(be, limit=600):
+    return be.make_rope_cache(limit, HD, 1e6)
+
+
+def check_append(be, s, qh, slots, token_pos, row_seq=None, aliases=False):
+    """One append against the plain form; everything it does not name stays bit for bit."""
+    import torch
+
+    n, kvh = len(slots), s.kvh
+    rope = tables(be)
+    wide = s.randn(n, qh + 2 * kvh, HD)
+    q, k, v = wide.split([qh, kvh, kvh], dim=1)
+    qn, kn = s.randn(HD), s.randn(HD)
+    pos = ints(token_pos).long().clamp(0, 599)
+    zq, tq = cu.turn(q, qn, rope.cosine[pos], rope.sine[pos], EPS)
+    zk, tk = cu.turn(k, kn, rope.cosine[pos], rope.sine[pos], EPS)
+    before = [x.clone() for x in (s.k, s.v, s.w, s.pos, wide)]
+    slot_t = ints(slots)
+    q_out = q if aliases else torch.full((n, qh, HD), 5.0, dtype=torch.bfloat16, device="cuda")
+    lens_out = slot_t if aliases else torch.full((n,), 99, dtype=torch.int32, device="cuda")
+    with s.cache() as cache:
+        be.cache_append(cache, q, k, v, qn, kn, rope, ints(token_pos), slot_t, q_out, EPS, lens_out=lens_out,
+                        row_seq=None if row_seq is None else ints(row_seq))
+        cache.sync()
+    wk, wv, ww, wp, ww_ = before
+    live = [i for i in range(n) if slots[i] >= 0]
+    for i in live:
+        seq = i if row_seq is None else row_seq[i]
+        page = int(s.tables[seq, slots[i] // PAGE])
+        at = slots[i] % PAGE
+        close(q_out[i], zq[i], tq[i], "query")
+        close(s.k[page, :, at], zk[i], tk[i], "key")
+        wk[page, :, at] = s.k[page, :, at]
+        wv[page, :, at] = v[i]
+        ww[seq, :, slots[i]] = 0.0
+        wp[seq, :, slots[i]] = token_pos[i]
+        assert int(lens_out[i]) == slots[i] + 1
+    for i in set(range(n)) - set(live):
+        assert int(lens_out[i]) == (slots[i] if aliases else 99)
+        if not aliases:
+            assert (q_out[i] == 5.0).all()
+    assert same(s.k, wk) and same(s.v, wv) and same(s.w, ww) and same(s.pos, wp)
+    if not aliases:
+        assert same(wide, ww_)
+
+
+@pytest.mark.parametrize("aliases", [False, True])
+@pytest.mark.parametrize("qh,kvh", [(8, 8), (32, 8), (64, 8), (4, 1), (15, 5), (1, 1)])
+def test_append(be, qh, kvh, aliases):
+    s = Setup(6, kvh, 200, seed=qh)
+    check_append(be, s, qh, [0, 199, 63, 64, -1, 130], [0, 599, 64, 63, 7, 1], aliases=aliases)
+
+
+def test_append_of_a_prompt(be):
+    """Many rows of few sequences, in any order."""
+    s = Setup(3, 2, 500, seed=11)
+    rng = np.random.default_rng(3)
+    seqs = rng.permutation([0] * 400 + [2] * 77).tolist()
+    order = {0: rng.permutation(500)[:400].tolist(), 2: rng.permutation(500)[:77].tolist()}
+    check_append(be, s, 4, [order[r].pop() for r in seqs], rng.integers(0, 600, 477).tolist(), row_seq=seqs)
+
+
+@pytest.mark.parametrize("what,row", [("slot", (200, 5, 0)), ("slot", (-2, 5, 0)), ("position", (3, 600, 0)),
+                                      ("position", (3, -1, 0)), ("sequence", (3, 5, 2)), ("sequence", (3, 5, -1)),
+                                      ("page", (70, 5, 1))])
+def test_append_refuses_bad_device_values(be, what, row):
+    """The row is left out, the others are written, the error is reported once."""
+    import torch
+
+    from inference_b200 import Q3Error
+
+    s = Setup(2, 2, 200, seed=12)
+    s.tables[1, 1] = s.k.shape[0] + 5
+    rope = tables(be)
+    slots, token_pos, seqs = [1, row[0]], [1, row[1]], [0, row[2]]
+    before = [x.clone() for x in (s.k, s.v, s.w, s.pos)]
+    q, k, v = s.randn(2, 4, HD), s.randn(2, 2, HD), s.randn(2, 2, HD)
+    qn = s.randn(HD)
+    q_out = torch.zeros_like(q)
+    lens_out = ints([0, 0])
+    with s.cache() as cache:
+        be.cache_append(cache, q, k, v, qn, qn, rope, ints(token_pos), ints(slots), q_out, EPS, lens_out=lens_out,
+                        row_seq=ints(seqs))
+        with pytest.raises(Q3Error) as e:
+            cache.sync()
+        assert e.value.status == 5 and what in str(e.value)
+        cache.sync()
+    page = int(s.tables[0, 0])
+    assert same(s.v[page, :, 1], v[0]) and lens_out.tolist() == [2, 0]
+    assert not q_out[1].any() and q_out[0].any()
+    for now, was in zip((s.k, s.v), before):
+        was[page, :, 1] = now[page, :, 1]
+        assert same(now, was)
+    assert same(s.w[1], before[2][1]) and same(s.pos[1], before[3][1])
+
+
+def fill_state(s, lens, seed, ties):
+    """Weights (with ties and special values) and distinct positions of each sequence's slots, in any order."""
+    rng = np.random.default_rng(seed)
+    w = np.exp(2.0 * rng.standard_normal(tuple(s.w.shape))).astype(np.float32)
+    if ties:
+        w = np.round(w).astype(np.float32)
+        w.reshape(-1)[rng.integers(0, w.size, w.size // 10)] = -0.0
+    p = np.zeros(w.shape, np.int32)
+    for r, n in enumerate(lens):
+        for h in range(w.shape[1]):
+            p[r, h, :n] = rng.permutation(n) + 10
+    s.w.copy_(cu.torch().from_numpy(w))
+    s.pos.copy_(cu.torch().from_numpy(p))
+    return w, p, [n + 10 for n in lens]
+
+
+def check_evict(be, s, lens, keep, recent, w, p, next_pos, in_place):
+    import torch
+
+    want_lens, moves = cu.evict(lens, next_pos, keep, recent, w, p)
+    before = [x.clone() for x in (s.k, s.v, s.w, s.pos)]
+    wk, wv, ww, wp = cu.apply_moves(s, moves, *before)
+    lens_t = ints(lens)
+    lens_out = lens_t if in_place else torch.full_like(lens_t, 77)
+    wo = po = None
+    if not in_place:
+        whole = (s.rows, s.kvh, s.w.stride(1))
+        wo = torch.full(whole, 3.0, device="cuda")[:, :, :s.max_len]
+        po = torch.full(whole, 3, dtype=torch.int32, device="cuda")[:, :, :s.max_len]
+    with s.cache() as cache:
+        be.cache_evict(cache, lens_t, ints(next_pos), keep, recent, lens_out, weights_out=wo, positions_out=po)
+        cache.sync()
+    assert lens_out.tolist() == want_lens
+    assert same(s.k, wk) and same(s.v, wv)
+    if in_place:
+        assert same(s.w, ww) and same(s.pos, wp)
+    else:
+        assert same(s.w, before[2]) and same(s.pos, before[3])
+        for r, n in enumerate(want_lens):
+            assert same(wo[r, :, :n], ww[r, :, :n]) and same(po[r, :, :n], wp[r, :, :n])
+            assert (wo[r, :, n:] == 3.0).all() and (po[r, :, n:] == 3).all()
+
+
+EVICT = [([65], 64, 0), ([65], 64, 64), ([1, 0, 5], 1, 0), ([300, 40, 301, 64, 1000], 64, 20),
+         ([1000, 999, 0, 500], 500, 499), ([1000, 700], 699, 900), ([5000, 1025, 1024], 1024, 100), ([20000], 333, 64),
+         ([33000, 2000], 30000, 1000), ([70], 1 << 19, 3)]
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("ties", [False, True])
+@pytest.mark.parametrize("lens,keep,recent", EVICT, ids=lambda v: str(v).replace(" ", ""))
+def test_evict(be, lens, keep, recent, ties, in_place):
+    s = Setup(len(lens), 3, max(max(lens), 1), seed=keep, slot_stride=max(lens) + 7)
+    w, p, next_pos = fill_state(s, lens, seed=sum(lens), ties=ties)
+    check_evict(be, s, lens, keep, recent, w, p, next_pos, in_place)
+
+
+def test_evict_equal_and_special_weights(be):
+    """All weights equal (ties by slot), NaN last, infinities and negatives in order, denormals, every slot recent."""
+    lens = [200] * 5
+    s = Setup(5, 1, 200, seed=21)
+    w, p, next_pos = fill_state(s, lens, seed=4, ties=False)
+    w[0] = 1.25
+    w[1, 0, ::3] = np.nan
+    w[2, 0, :6] = [np.inf, -np.inf, -1.0, 0.0, -0.0, 1e-42]
+    w[2, 0, 6:] = np.float32(1e-41)
+    w[3] = np.nan
+    s.w.copy_(cu.torch().from_numpy(w))
+    next_pos[4] = 0  # every position is recent
+    check_evict(be, s, lens, 100, 0, w, p, next_pos, True)
+
+
+def test_evict_refuses_bad_device_values(be):
+    """A bad length or page leaves its sequence as it was and is reported; the others shrink."""
+    import torch
+
+    from inference_b200 import Q3Error
+
+    for bad in ("length", "page"):
+        lens = [150, 150, 150]
+        s = Setup(3, 2, 150, seed=22)
+        w, p, next_pos = fill_state(s, lens, seed=5, ties=False)
+        if bad == "page":
+            s.tables[1, 2] = -7
+        given = ints([150, 151 if bad == "length" else 150, 150])
+        before = [x.clone() for x in (s.k, s.v, s.w, s.pos)]
+        ok = Setup(3, 2, 150, seed=22)
+        _, moves = cu.evict([150, 0, 150], next_pos, 64, 10, w, p)
+        want = cu.apply_moves(ok, moves, *before)
+        with s.cache() as cache:
+            be.cache_evict(cache, given, ints(next_pos), 64, 10, given)
+            with pytest.raises(Q3Error) as e:
+                cache.sync()
+            assert e.value.status == 5 and bad in str(e.value)
+        assert given.tolist() == [64, 151 if bad == "length" else 150, 64]
+        for now, expect in zip((s.k, s.v, s.w, s.pos), want):
+            assert same(now, expect)
+        torch.cuda.synchronize()
+
+
+def test_bounded_decode_loop(be):
+    """Append, attend, evict as a user runs them: sequences of different lengths decode past their budget.  Every step's
+    output is held to the 64-bit form over the slots that the plain form of the earlier evictions left (chosen by the
+    weights that the cache reports), and each slot's position says which token it holds."""
+    import torch
+
+    qh, kvh, keep, recent, cap, steps = 8, 2, 96, 32, 112, 60
+    start = [90, 3, 0]
+    s = Setup(3, kvh, cap, seed=31)
+    rope = tables(be)
+    qn, kn = s.randn(HD), s.randn(HD)
+    s.w.zero_()
+    keys, values = {}, {}  # (row, position) -> the token's stored key and value rows
+    lens = ints(start)
+    next_pos = ints(start)
+    for r, n in enumerate(start):
+        for h in range(kvh):
+            s.pos[r, h, :n] = torch.arange(n, dtype=torch.int32, device="cuda")
+        for j in range(n):
+            page = int(s.tables[r, j // PAGE])
+            keys[r, j], values[r, j] = s.k[page, :, j % PAGE].clone(), s.v[page, :, j % PAGE].clone()
+    with s.cache() as cache:
+        for step in range(steps):
+            wide = s.randn(3, qh + 2 * kvh, HD)
+            q, k, v = wide.split([qh, kvh, kvh], dim=1)
+            q_out = torch.empty(3, qh, HD, dtype=torch.bfloat16, device="cuda")
+            slots = lens.clone()
+            be.cache_append(cache, q, k, v, qn, kn, rope, next_pos, lens, q_out, EPS, lens_out=lens)
+            now = lens.tolist()
+            for r in range(3):
+                at = int(slots[r])
+                page = int(s.tables[r, at // PAGE])
+                pos = int(next_pos[r])
+                keys[r, pos], values[r, pos] = s.k[page, :, at % PAGE].clone(), s.v[page, :, at % PAGE].clone()
+            check_attention(be, s, cache, q_out, now)
+            next_pos += 1
+            if step % 5 == 4:
+                w, p = s.w.cpu().numpy(), s.pos.cpu().numpy()
+                want_lens, moves = cu.evict(now, next_pos.tolist(), keep, recent, w, p)
+                want = cu.apply_moves(s, moves, s.k, s.v, s.w, s.pos)
+                be.cache_evict(cache, lens, next_pos, keep, recent, lens)
+                cache.sync()
+                assert lens.tolist() == want_lens
+                assert all(same(a, b) for a, b in zip((s.k, s.v, s.w, s.pos), want))
+        lens_now = lens.tolist()
+    assert lens_now == [keep, 63, 60]
+    for r, n in enumerate(lens_now):
+        for h in range(kvh):
+            held = s.pos[r, h, :n].tolist()
+            assert len(set(held)) == n and set(range(int(next_pos[r]) - recent, int(next_pos[r]))) <= set(held)
+            for j, pos in enumerate(held):
+                page = int(s.tables[r, j // PAGE])
+                assert same(s.k[page, h, j % PAGE], keys[r, pos][h]) and same(s.v[page, h, j % PAGE], values[r, pos][h])
+
+
+def test_captured_step_replays(be):
+    """One step of the three calls as a CUDA graph: two graphs on the same cache, replayed in turn with lengths and
+    positions that advance on the device, against the same calls made one by one."""
+    import torch
+
+    qh, kvh, keep, recent, cap = 8, 2, 70, 16, 80
+    rope = tables(be)
+
+    def state():
+        s = Setup(3, kvh, cap, seed=41)
+        s.w.zero_()
+        s.pos.copy_(torch.arange(cap, dtype=torch.int32, device="cuda").expand(3, kvh, cap))
+        s.lens, s.next = ints([69, 70, 12]), ints([69, 70, 12])
+        s.q = [s.randn(3, qh, HD) for _ in range(2)]
+        s.kv = [(s.randn(3, kvh, HD), s.randn(3, kvh, HD)) for _ in range(2)]
+        s.qn, s.out = s.randn(HD), [torch.zeros(3, qh, HD, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        return s
+
+    def step(s, cache, i):
+        q_out = torch.empty_like(s.q[i])
+        be.cache_append(cache, s.q[i], *s.kv[i], s.qn, s.qn, rope, s.next, s.lens, q_out, EPS, lens_out=s.lens)
+        be.cache_attention(cache, q_out, s.lens, s.out[i])
+        s.next.add_(1)
+        be.cache_evict(cache, s.lens, s.next, keep, recent, s.lens)
+
+    a, b = state(), state()
+    with a.cache() as ca, b.cache() as cb:
+        side = torch.cuda.Stream()
+        graphs = []
+        with torch.cuda.stream(side):
+            for i in range(2):
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=side):
+                    step(b, cb, i)
+                graphs.append(g)
+        torch.cuda.synchronize()
+        for n in range(6):
+            step(a, ca, n % 2)
+            graphs[n % 2].replay()
+            torch.cuda.synchronize()
+            for x, y in zip((a.k, a.v, a.w, a.pos, a.lens, a.out[0], a.out[1]),
+                            (b.k, b.v, b.w, b.pos, b.lens, b.out[0], b.out[1])):
+                assert same(x, y), n
+        ca.sync()
+        cb.sync()
+        del graphs
+
+
+def test_calls_on_two_streams(be):
+    """Two caches, each on its own stream, at the same time: the same results as one after the other."""
+    import torch
+
+    lens = [3000, 100, 64]
+    sets = [Setup(3, 4, 3000, seed=51 + i) for i in range(2)]
+    qs = [s.randn(3, 16, HD) for s in sets]
+    alone, start = [], [s.w.clone() for s in sets]
+    caches = [s.cache() for s in sets]
+    for s, q, c in zip(sets, qs, caches):
+        out = torch.empty_like(q)
+        be.cache_attention(c, q, ints(lens), out)
+        c.sync()
+        alone.append((out, s.w.clone()))
+    streams = [torch.cuda.Stream() for _ in sets]
+    lens_t = ints(lens)
+    for _ in range(5):
+        for s, w in zip(sets, start):
+            s.w.copy_(w)
+        outs = [torch.zeros_like(q) for q in qs]
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                be.cache_attention(caches[i], qs[i], lens_t, outs[i])
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert same(outs[i], alone[i][0]) and same(sets[i].w, alone[i][1])
+    for c in caches:
+        c.close()
