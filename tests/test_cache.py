@@ -134,3 +134,15 @@ def test_python_handle_refuses_cpu_tensors():
     k = torch.zeros(2, 1, 64, 128, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="CUDA"):
         PagedCache(k, k.clone(), torch.zeros(1, 1, dtype=torch.int32))
+
+
+def test_work_shares(tmp_path):
+    """The shares of the attention's work, from lengths in any state, against a walk over every tile."""
+    import os
+    import subprocess
+
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cache_plan_check.cpp")
+    exe = str(tmp_path / "cache_plan_check")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=address,undefined", "-o", exe, src], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
