@@ -475,10 +475,12 @@ Q3_API int q3_batch_info(q3_batch* b, uint32_t seq, size_t* position, size_t* fr
  * them.  Values in device memory that are out of range
  * (a page outside the pool, a length or slot past max_len, a position past the
  * RoPE tables) are never followed: the row is skipped (attention: its output is
- * NaN) and q3_cache_sync reports Q3_ERR_DEVICE.
+ * NaN) and q3_cache_sync reports Q3_ERR_DEVICE.  Calls on one cache change it:
+ * the caller orders them (one stream, or events).
  * ---------------------------------------------------------------------- */
 typedef struct q3_cache q3_cache;
 
+#define Q3_CACHE_STATE_WORDS 4
 typedef struct q3_cache_desc {
     uint16_t* k_pages_dev; /* [num_pages, kv_heads, page_size, head_dim] */
     uint16_t* v_pages_dev;
@@ -493,7 +495,9 @@ typedef struct q3_cache_desc {
     size_t kv_heads;
     size_t head_dim;  /* 128 */
     size_t page_size; /* 64 */
-    uint32_t* error_dev; /* one word, 0 at first: the first error that a kernel of this cache met */
+    uint32_t* state_dev; /* Q3_CACHE_STATE_WORDS words, 0 at first and the library's from then on:
+                          * the first error that a kernel of this cache met, and the attention's
+                          * work counter */
 } q3_cache_desc;
 
 /* The handle works on `device`, whichever device is current when it is used.
@@ -501,7 +505,7 @@ typedef struct q3_cache_desc {
 Q3_API int q3_cache_create(const q3_cache_desc* desc, int device, q3_cache** out);
 Q3_API int q3_cache_destroy(q3_cache* c);
 
-/* Blocks until `stream` has finished, then reports (and clears) the error word:
+/* Blocks until `stream` has finished, then reports (and clears) an error:
  * Q3_ERR_DEVICE with its cause if a kernel recorded one. */
 Q3_API int q3_cache_sync(q3_cache* c, void* stream);
 
@@ -530,7 +534,7 @@ Q3_API int q3_cache_append(q3_cache* c, const uint16_t* q_dev, size_t q_stride, 
  * sequence of length 0 gets zeros and keeps its weights.  out may be q (with
  * its stride).  Strides in elements, multiples of 8.  The workspace (16-byte
  * aligned, q3_cache_attention_workspace_bytes) belongs to the call until it has
- * finished on the GPU; calls on unordered streams need one each. */
+ * finished on the GPU; unordered calls on different caches need one each. */
 Q3_API size_t q3_cache_attention_workspace_bytes(const q3_cache* c, size_t q_heads, int accumulate);
 Q3_API int q3_cache_attention(q3_cache* c, const uint16_t* q_dev, size_t q_stride, const int32_t* lens_dev,
                               uint16_t* out_dev, size_t out_stride, size_t q_heads, int accumulate,

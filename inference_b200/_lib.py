@@ -156,7 +156,7 @@ class CacheDesc(C.Structure):
                 ("page_tables", C.c_void_p), ("table_stride", C.c_size_t), ("weights", C.c_void_p),
                 ("positions", C.c_void_p), ("slot_stride", C.c_size_t), ("rows", C.c_size_t),
                 ("max_len", C.c_size_t), ("kv_heads", C.c_size_t), ("head_dim", C.c_size_t),
-                ("page_size", C.c_size_t), ("error", C.c_void_p)]
+                ("page_size", C.c_size_t), ("state", C.c_void_p)]
 
 
 WEIGHT_FORMATS = {"bf16": 0, "fp8": 1, "nvfp4": 2}  # Q3_WEIGHTS_BF16, Q3_WEIGHTS_FP8_E4M3, Q3_WEIGHTS_NVFP4

@@ -19,7 +19,8 @@ class PagedCache:
 
     weights and positions may both be None (no accumulation, no eviction).
     max_len, the slots a sequence may hold, defaults to what the page tables and
-    weights cover.  The handle keeps the tensors alive."""
+    weights cover.  The handle keeps the tensors alive.  Calls on one cache are
+    ordered by the caller: one stream, or events."""
 
     def __init__(self, k_pages, v_pages, page_tables, weights=None, positions=None, max_len: int | None = None):
         import torch
@@ -53,17 +54,17 @@ class PagedCache:
         self.k_pages, self.v_pages, self.page_tables = k_pages, v_pages, page_tables
         self.weights, self.positions = weights, positions
         self.device, self.rows, self.kv_heads, self.max_len = dev, rows, kvh, max_len
-        self.error = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.state = torch.zeros(4, dtype=torch.int32, device=dev)
         d = CacheDesc(k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], page_tables.data_ptr(),
                       page_tables.stride(0) if rows > 1 else page_tables.shape[1],
                       weights.data_ptr() if weights is not None else None,
                       positions.data_ptr() if positions is not None else None,
                       weights.stride(1) if weights is not None else 0, rows, max_len, kvh, k_pages.shape[3],
-                      k_pages.shape[2], self.error.data_ptr())
+                      k_pages.shape[2], self.state.data_ptr())
         h = C.c_void_p()
         check(lib().q3_cache_create(C.byref(d), dev.index, C.byref(h)))
         self.h = h
-        # the zeroed error word is there before any stream's kernels can reach it
+        # the zeroed state is there before any stream's kernels can reach it
         torch.cuda.current_stream(dev).synchronize()
 
     @staticmethod

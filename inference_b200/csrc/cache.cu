@@ -140,12 +140,15 @@ extern "C" {
 int q3_cache_create(const q3_cache_desc* d, int device, q3_cache** out) {
     Q3_CHECK(d && out, "q3_cache_create: null argument");
     *out = nullptr;
-    Q3_CHECK(d->k_pages_dev && d->v_pages_dev && d->page_tables_dev && d->error_dev, "q3_cache_create: null pointer");
+    Q3_CHECK(d->k_pages_dev && d->v_pages_dev && d->page_tables_dev && d->state_dev, "q3_cache_create: null pointer");
     if (d->head_dim != kCacheHd) return fail(Q3_ERR_UNSUPPORTED, "q3_cache_create: head_dim must be 128");
     if (d->page_size != kCachePage) return fail(Q3_ERR_UNSUPPORTED, "q3_cache_create: page_size must be 64");
     Q3_CHECK(d->kv_heads >= 1 && d->kv_heads <= 1024, "q3_cache_create: kv_heads must be 1 .. 1024");
     Q3_CHECK(d->rows >= 1 && d->rows <= 4096, "q3_cache_create: rows must be 1 .. 4096");
     Q3_CHECK(d->max_len >= 1 && d->max_len <= (1u << 20), "q3_cache_create: max_len must be 1 .. 2^20");
+    // tiles of 64 slots are numbered in 32 bits, all sequences' heads together
+    Q3_CHECK(d->rows * d->kv_heads * ((d->max_len + kCachePage - 1) / kCachePage) <= INT_MAX,
+             "q3_cache_create: rows * kv_heads * ceil(max_len / 64) must be below 2^31");
     // rows of the pools are addressed by 32-bit tensor-map coordinates
     Q3_CHECK(d->num_pages >= 1 && d->num_pages <= INT_MAX / (kCachePage * d->kv_heads),
              "q3_cache_create: num_pages * kv_heads * 64 must be below 2^31");
@@ -157,8 +160,8 @@ int q3_cache_create(const q3_cache_desc* d, int device, q3_cache** out) {
              "q3_cache_create: slot_stride must be at least max_len");
     Q3_CHECK(aligned(d->k_pages_dev, 16) && aligned(d->v_pages_dev, 16), "q3_cache_create: 16-byte aligned pages required");
     Q3_CHECK(aligned(d->page_tables_dev, 4) && aligned(d->weights_dev, 4) && aligned(d->positions_dev, 4) &&
-                 aligned(d->error_dev, 4),
-             "q3_cache_create: 4-byte aligned tables, weights, positions and error word required");
+                 aligned(d->state_dev, 4),
+             "q3_cache_create: 4-byte aligned tables, weights, positions and state required");
     Q3_CHECK(device >= 0, "q3_cache_create: bad device");
     auto* c = new (std::nothrow) q3_cache();
     if (!c) return fail(Q3_ERR_OOM, "q3_cache_create: host allocation failed");
@@ -176,7 +179,8 @@ int q3_cache_create(const q3_cache_desc* d, int device, q3_cache** out) {
     v.rows = static_cast<int>(d->rows);
     v.max_len = static_cast<int>(d->max_len);
     v.kv_heads = static_cast<int>(d->kv_heads);
-    v.err = d->error_dev;
+    v.err = d->state_dev;
+    v.next_chunk = d->state_dev + 1;
     *out = c;
     return Q3_OK;
 }

@@ -21,7 +21,7 @@ struct CacheView {
     int32_t* positions;
     long long slot_stride;
     int rows, max_len, kv_heads;
-    uint32_t* err;
+    uint32_t *err, *next_chunk;  // q3_cache_desc.state_dev: the error word; chunks taken by the attention running
 };
 
 __host__ __device__ inline size_t cache_slot_index(const CacheView& c, int row, int head) {

@@ -6,21 +6,21 @@
 //
 // Bound: HBM.  K and V of every slot cross it once (512 bytes a slot and kv head)
 // for 512 G flops; everything else is two orders smaller.  So:
-//   * all sequences' 64-slot tiles are cut into equal shares (cache_plan.hpp), one
-//     per resident CTA (two an SM), from the lengths in device memory: one launch
-//     shape serves any mix of lengths, and no SM waits for the longest sequence;
+//   * all sequences' 64-slot tiles are cut into chunks (cache_plan.hpp) from the
+//     lengths in device memory, so one launch shape serves any mix of lengths; two
+//     CTAs an SM take chunks as they become free;
 //   * in a CTA one warp streams K and V tiles through a ring of 32 KB stages by
 //     swizzled 2-D TMA (a last, partial tile by boxes of 16 slots), reading page
 //     table entries for 32 tiles at a time; four warps take 16 slots of a tile
 //     each: S^T = K Q^T and O^T += V^T P^T on the tensor cores with the slots as
 //     M and the group's query heads as N, online softmax in fp32, P as the sum of
 //     two BF16 parts (2^-16 of its size);
-//   * a run (sequence, kv head) within one share is finished by it; parts of a cut
+//   * a run (sequence, kv head) within one chunk is finished there; parts of a cut
 //     run (maximum, sum, unnormalised output in fp32) are joined by the second
-//     kernel in share order, so results do not depend on timing;
+//     kernel in chunk order, so results do not depend on timing;
 //   * probabilities need the run's final maximum and sum: the first kernel leaves
 //     the raw scores (fp32, 4 G bytes a slot, written once and mostly read back
-//     from L2), the second turns them into weights, share by share.
+//     from L2), the second turns them into weights.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -36,17 +36,17 @@ constexpr int kWarps = 4;                      // consumer warps, 16 slots of a 
 constexpr int kConsumers = kWarps * 32;
 constexpr int kThreads = kConsumers + 32;      // + producer warp
 constexpr int kTileBytes = kCachePage * kCacheHd * 2;
-constexpr int kJoinThreads = 512;
-constexpr int kAccPitch = 68;                  // floats of a head's 64 dims in the merge buffer: conflict-free
+constexpr int kAccPitch = kCacheHd + 4;         // floats of a head in the merge buffer: conflict-free
 constexpr float kScoreScale = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
 
 // What the producer tells the consumers about a stage's tile.
 enum : int {
-    TILE_FIRST = 1,  // first tile of its run in this share
-    TILE_LAST = 2,   // last tile of its run in this share
-    TILE_WHOLE = 4,  // the run lies in this share
-    TILE_BEGIN = 8,  // the run begins in this share
+    TILE_FIRST = 1,  // first tile of its run in this chunk
+    TILE_LAST = 2,   // last tile of its run in this chunk
+    TILE_WHOLE = 4,  // the run lies in this chunk
+    TILE_BEGIN = 8,  // the run begins in this chunk
     TILE_BAD = 16,   // its page lies outside the pool: nothing was loaded
+    TILE_END = 32,   // no tile: the CTA is done
 };
 
 // NT: 8-head column tiles (1: up to 8 query heads per kv head, 2: up to 16).
@@ -59,32 +59,33 @@ struct Cfg {
 
 template <int NT>
 struct Smem {
-    uint8_t ring[Cfg<NT>::kStages][Cfg<NT>::kStageBytes];  // K tile, V tile, the run's queries (first tile only)
-    float acc[kWarps][Cfg<NT>::kHeads][kAccPitch];         // 64 dims of every warp's output, merging
+    // K tile, V tile, the run's queries (first tile only); after a run's last tile the
+    // stage is where the warps' outputs meet ([warp][head][kAccPitch] floats)
+    uint8_t ring[Cfg<NT>::kStages][Cfg<NT>::kStageBytes];
     float m[kWarps][Cfg<NT>::kHeads], l[kWarps][Cfg<NT>::kHeads];
-    float f[kWarps][Cfg<NT>::kHeads];                      // a warp's weight in the merge
-    float cm[Cfg<NT>::kHeads], cl[Cfg<NT>::kHeads];
-    int4 tile[Cfg<NT>::kStages];                           // row, head, live slots, flags
+    int4 tile[Cfg<NT>::kStages];        // row, head, tile, flags | live slots << 8 | chunk << 16
     uint64_t full[Cfg<NT>::kStages], empty[Cfg<NT>::kStages];
-    uint64_t meet;                                         // the consumer warps' barrier in a merge
-    int chunk[kThreads + 1];                               // tiles before each chunk of rows
+    Plan plan;
+    int before[kThreads + 1];           // tiles before each group of rows
     int scan[kThreads / 32];
 };
+static_assert(kWarps * Cfg<1>::kHeads * kAccPitch * 4 <= Cfg<1>::kStageBytes, "merge buffer");
+static_assert(kWarps * Cfg<2>::kHeads * kAccPitch * 4 <= Cfg<2>::kStageBytes, "merge buffer");
 
 struct Parts {
-    float2* ml;    // [rows][q_heads]: maximum (log2) and sum of runs within one share
-    float2* pml;   // [shares][2][heads]: of parts
-    float* po;     // [shares][2][heads][128]: unnormalised outputs of parts
+    float2* ml;    // [rows][q_heads]: maximum (log2) and 1 / sum of runs within one chunk (0: a bad page)
+    float2* pml;   // [chunks][2][heads]: maximum and sum of parts
+    float* po;     // [chunks][2][heads][128]: unnormalised outputs of parts
     float* score;  // [tile][64][G]: raw scores in log2 units
-    int shares, heads;
+    int workers, heads;
 };
 
-// Chunks of consecutive rows, one per thread: chunk[t] = tiles (of one kv head)
-// before thread t's rows, chunk[threads] = all.
+// Groups of consecutive rows, one per thread: before[t] = tiles (of one kv head)
+// before thread t's rows, before[threads] = all.
 template <int THREADS>
-__device__ __forceinline__ void scan_rows(const int32_t* lens, const CacheView& c, int* chunk, int* scan) {
+__device__ __forceinline__ void scan_rows(const int32_t* lens, const CacheView& c, int* before, int* scan) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int per = plan_chunk_rows(c.rows, THREADS);
+    const int per = plan_group_rows(c.rows, THREADS);
     int sum = 0;
     for (int r = tid * per; r < min(c.rows, tid * per + per); ++r) sum += plan_tiles(lens[r], c.max_len);
     int incl = sum;
@@ -95,16 +96,32 @@ __device__ __forceinline__ void scan_rows(const int32_t* lens, const CacheView& 
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    int before = 0;
-    for (int i = 0; i < warp; ++i) before += scan[i];
-    chunk[tid + 1] = before + incl;
-    if (tid == 0) chunk[0] = 0;
+    for (int i = 0; i < warp; ++i) incl += scan[i];
+    before[tid + 1] = incl;
+    if (tid == 0) before[0] = 0;
     __syncthreads();
 }
 
 template <int THREADS>
-__device__ __forceinline__ PlanPlace locate(long long t, const int32_t* lens, const CacheView& c, const int* chunk) {
-    return plan_locate(t, lens, c.rows, c.max_len, c.kv_heads, chunk, THREADS);
+__device__ __forceinline__ PlanPlace locate(int t, const int32_t* lens, const CacheView& c, const int* before) {
+    return plan_locate(t, lens, c.rows, c.max_len, c.kv_heads, before, THREADS);
+}
+
+// The consumer warps meet; whether all of them say yes.
+__device__ __forceinline__ bool consumers_all(bool yes) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, 1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"(static_cast<uint32_t>(yes)), "n"(kConsumers)
+        : "memory");
+    return all != 0;
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
 __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar, uint64_t policy) {
@@ -122,90 +139,88 @@ struct Maps {
 };
 
 template <int NT>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __maxnreg__(NT == 1 ? 128 : 168)
     cache_attention_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ Maps maps, const Parts parts) {
     using C = Cfg<NT>;
     constexpr int S = C::kStages;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const CacheView& c = a.c;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.q_heads / c.kv_heads;
-    if (tid == 0) {
+    pdl_trigger();  // the joining kernel may set itself up; it waits for this one's end
+    if (tid == kConsumers) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&sm.full[s], 1);
             mbar_init(&sm.empty[s], kWarps);
         }
-        mbar_init(&sm.meet, kWarps);
         fence_barrier_init();
+        prefetch_map(&maps.k64);
+        prefetch_map(&maps.v64);
+        prefetch_map(&maps.k16);
+        prefetch_map(&maps.v16);
     }
-    scan_rows<kThreads>(a.lens, c, sm.chunk, sm.scan);
-    pdl_trigger();  // the joining kernel may set itself up; it waits for this one's end
-    const long long total = static_cast<long long>(sm.chunk[kThreads]) * c.kv_heads;
-    const int shares = plan_shares(total, parts.shares);
-    const long long t0 = plan_first(total, shares, b);
-    const int n = b < shares ? static_cast<int>(plan_first(total, shares, b + 1) - t0) : 0;
-
-    // sequences without a tile: length 0 gives zeros, a length out of range NaN
-    for (int r = b; r < c.rows; r += gridDim.x) {
-        const int len = a.lens[r];
-        if (len > 0 && len <= c.max_len) continue;
-        if (len != 0 && tid == 0) record_error(c.err, DEV_BAD_LENGTH);
-        const uint32_t v = len == 0 ? 0u : 0x7FC07FC0u;
-        uint4* o = reinterpret_cast<uint4*>(a.out + r * a.out_stride);
-        for (int i = tid; i < a.q_heads * kCacheHd / 8; i += kThreads) o[i] = make_uint4(v, v, v, v);
-    }
-    if (n == 0) return;
+    scan_rows<kThreads>(a.lens, c, sm.before, sm.scan);
 
     if (warp == kWarps) {
         // ------------------------------------------------------------ producer
+        if (lane == 0) plan_make(sm.plan, sm.before[kThreads] * c.kv_heads, parts.workers);
+        __syncwarp();
+        const Plan& plan = sm.plan;
         const uint64_t pol = policy_evict_first();
-        int issued = 0;
-        bool stop = false;
-        for (int i0 = 0; i0 < n && !stop; i0 += 32) {
-            // lane i: tile i0 + i
-            int4 d = make_int4(0, 0, 0, 0);
-            int y = 0;
-            if (i0 + lane < n) {
-                const long long t = t0 + i0 + lane;
-                const PlanPlace p = locate<kThreads>(t, a.lens, c, sm.chunk);
-                const long long run0 = t - p.tile;
-                const bool begins = run0 >= t0, ends = run0 + p.tiles <= t0 + n;
-                const int page = c.tables[p.row * c.table_stride + p.tile];
-                int flags = 0;
-                if (p.tile == 0 || i0 + lane == 0) flags |= TILE_FIRST;
-                if (p.tile == p.tiles - 1 || i0 + lane == n - 1) flags |= TILE_LAST;
-                if (begins && ends) flags |= TILE_WHOLE;
-                if (begins) flags |= TILE_BEGIN;
-                if (page < 0 || page >= c.num_pages) {
-                    flags |= TILE_BAD;
-                    record_error(c.err, DEV_BAD_PAGE);
-                } else {
-                    y = (page * c.kv_heads + p.head) * kCachePage;
+        int k = 0;        // tiles issued
+        bool ok = true;
+        // a stage to fill: the k-th
+        auto stage_free = [&]() {
+            if (k < S) return true;
+            return mbar_wait(&sm.empty[k % S], ((k / S) - 1) & 1, c.err, DEV_TMA_WAIT_TIMEOUT);
+        };
+        int chunk = blockIdx.x;
+        while (ok && chunk < plan.chunks) {
+            // the chunk after this one, asked for ahead: whoever is free first takes the next
+            int next = plan.chunks;
+            if (lane == 0 && plan.chunks > gridDim.x) next = gridDim.x + static_cast<int>(atomicAdd(c.next_chunk, 1u));
+            int t0, t1;
+            plan_chunk(plan, chunk, t0, t1);
+            for (int i0 = t0; i0 < t1 && ok; i0 += 32) {
+                // lane i: tile i0 + i
+                int4 d = make_int4(0, 0, 0, 0);
+                int y = 0;
+                if (i0 + lane < t1) {
+                    const int t = i0 + lane;
+                    const PlanPlace p = locate<kThreads>(t, a.lens, c, sm.before);
+                    const int page = c.tables[p.row * c.table_stride + p.tile];
+                    const int run0 = t - p.tile;
+                    const bool begins = run0 >= t0, ends = run0 + p.tiles <= t1;
+                    int flags = 0;
+                    if (p.tile == 0 || t == t0) flags |= TILE_FIRST;
+                    if (p.tile == p.tiles - 1 || t == t1 - 1) flags |= TILE_LAST;
+                    if (begins && ends) flags |= TILE_WHOLE;
+                    if (begins) flags |= TILE_BEGIN;
+                    if (page < 0 || page >= c.num_pages) {
+                        flags |= TILE_BAD;
+                        record_error(c.err, DEV_BAD_PAGE);
+                    } else {
+                        y = (page * c.kv_heads + p.head) * kCachePage;
+                    }
+                    d = make_int4(p.row, p.head, t, flags | min(kCachePage, p.len - p.tile * kCachePage) << 8 | chunk << 16);
                 }
-                d = make_int4(p.row, p.head, min(kCachePage, p.len - p.tile * kCachePage), flags);
-            }
-            for (int i = 0; i < 32 && i0 + i < n; ++i) {
-                const int4 t = make_int4(__shfl_sync(0xffffffffu, d.x, i), __shfl_sync(0xffffffffu, d.y, i),
-                                         __shfl_sync(0xffffffffu, d.z, i), __shfl_sync(0xffffffffu, d.w, i));
-                const int row0 = __shfl_sync(0xffffffffu, y, i);
-                const int k = i0 + i, s = k % S;
-                int ok = 1;
-                if (lane == 0) {
-                    if (k >= S) ok = mbar_wait(&sm.empty[s], ((k / S) - 1) & 1, c.err, DEV_TMA_WAIT_TIMEOUT);
-                    if (ok) {
-                        sm.tile[s] = t;
-                        uint8_t* st = sm.ring[s];
-                        if (t.w & TILE_BAD) {
+                for (int i = 0; i < 32 && i0 + i < t1 && ok; ++i, ++k) {
+                    const int4 t = make_int4(__shfl_sync(0xffffffffu, d.x, i), __shfl_sync(0xffffffffu, d.y, i),
+                                             __shfl_sync(0xffffffffu, d.z, i), __shfl_sync(0xffffffffu, d.w, i));
+                    const int row0 = __shfl_sync(0xffffffffu, y, i);
+                    if (lane == 0) {
+                        ok = stage_free();
+                        const int s = k % S;
+                        if (ok && (t.w & TILE_BAD)) {
+                            sm.tile[s] = t;
                             mbar_arrive(&sm.full[s]);
-                        } else {
-                            const int boxes = (t.z + 15) / 16;  // of 16 slots
+                        } else if (ok) {
+                            sm.tile[s] = t;
+                            uint8_t* st = sm.ring[s];
+                            const int boxes = (((t.w >> 8) & 127) + 15) / 16;  // of 16 slots
                             const uint32_t q_bytes = (t.w & TILE_FIRST) ? G * kCacheHd * 2 : 0;
                             mbar_arrive_expect_tx(&sm.full[s], boxes * (2 * 16 * kCacheHd * 2) + q_bytes);
-                            if (q_bytes)
-                                bulk_g2s(st + 2 * kTileBytes,
-                                         a.q + t.x * a.q_stride + static_cast<size_t>(t.y) * G * kCacheHd, q_bytes,
-                                         &sm.full[s], pol);
                             if (boxes == 4) {
                                 for (int h = 0; h < 2; ++h) {
                                     tma_tile(st + h * 8192, &maps.k64, h * 64, row0, &sm.full[s], pol);
@@ -219,21 +234,39 @@ __global__ void __launch_bounds__(kThreads, 2)
                                         tma_tile(to + kTileBytes, &maps.v16, h * 64, row0 + 16 * x, &sm.full[s], pol);
                                     }
                             }
+                            if (q_bytes)
+                                bulk_g2s(st + 2 * kTileBytes,
+                                         a.q + t.x * a.q_stride + static_cast<size_t>(t.y) * G * kCacheHd, q_bytes,
+                                         &sm.full[s], pol);
                         }
                     }
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) --k;
                 }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-                if (!ok) {
-                    stop = true;
-                    break;
-                }
-                issued = k + 1;
+            }
+            chunk = __shfl_sync(0xffffffffu, next, 0);
+        }
+        if (lane == 0) {
+            ok = ok && stage_free();
+            if (ok) {
+                sm.tile[k % S].w = TILE_END;
+                mbar_arrive(&sm.full[k % S]);
+            } else {
+                // a wait ran out: leave no copy in flight behind
+                for (int i = max(0, k - S); i < k; ++i) mbar_wait(&sm.full[i % S], (i / S) & 1, nullptr, 0);
             }
         }
-        // leave no copy in flight behind a wait that ran out
-        if (stop && lane == 0)
-            for (int k = max(0, issued - S); k < issued; ++k) mbar_wait(&sm.full[k % S], (k / S) & 1, nullptr, 0);
         return;
+    }
+
+    // sequences without a tile: length 0 gives zeros, a length out of range NaN
+    for (int r = blockIdx.x; r < c.rows; r += gridDim.x) {
+        const int len = a.lens[r];
+        if (len > 0 && len <= c.max_len) continue;
+        if (len != 0 && tid == 0) record_error(c.err, DEV_BAD_LENGTH);
+        const uint32_t v = len == 0 ? 0u : 0x7FC07FC0u;
+        uint4* o = reinterpret_cast<uint4*>(a.out + r * a.out_stride);
+        for (int i = tid; i < a.q_heads * kCacheHd / 8; i += kConsumers) o[i] = make_uint4(v, v, v, v);
     }
 
     // ---------------------------------------------------------------- consumers
@@ -242,20 +275,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     float o[NT][8][4];                       // O^T: dims 16 dt + g (+ 8), heads 8 nt + 2 t4 (+ 1)
     float m_run[NT][2], l_run[NT][2];        // of those heads: maximum (log2), this lane's share of the sum
     bool poisoned = false;
-    // All four warps meet here in a merge.  An mbarrier, so that no wait is unbounded: a
-    // warp whose wait ran out returns, and the others' waits run out in turn.
-    uint32_t meet_phase = 0;
-    auto meet = [&]() {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.meet);
-        const bool ok = mbar_wait(&sm.meet, meet_phase, c.err, DEV_TMA_WAIT_TIMEOUT);
-        meet_phase ^= 1;
-        return ok;
-    };
-    for (int k = 0; k < n; ++k) {
+    for (int k = 0;; ++k) {
         const int s = k % S;
-        if (!mbar_wait(&sm.full[s], (k / S) & 1, c.err, DEV_TMA_WAIT_TIMEOUT)) return;
+        // all four warps go on or none: a wait that ran out in one of them ends them all
+        if (!consumers_all(mbar_wait(&sm.full[s], (k / S) & 1, c.err, DEV_TMA_WAIT_TIMEOUT))) return;
         const int4 d = sm.tile[s];
+        if (d.w & TILE_END) return;
         uint8_t* kt = sm.ring[s];
         uint8_t* vt = kt + kTileBytes;
         if (d.w & TILE_FIRST) {
@@ -276,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
         }
         if (d.w & TILE_BAD) poisoned = true;
-        const int valid = d.z;
+        const int valid = (d.w >> 8) & 127;
         bool wrote = false;
         if (warp * 16 < valid && !(d.w & TILE_BAD)) {
             if (valid < warp * 16 + 16) {
@@ -313,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 for (int e = 0; e < 4; ++e)
                     sc[e] = tok + (e >> 1) * 8 < valid ? (sa[nt][e] + sb[nt][e]) * kScoreScale : -INFINITY;
                 if (a.accumulate) {
-                    float* to = parts.score + ((t0 + k) * kCachePage + tok) * G + h0;
+                    float* to = parts.score + (static_cast<size_t>(d.z) * kCachePage + tok) * G + h0;
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
                         if (tok + 8 * r < valid) {
@@ -373,15 +398,12 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
             }
         }
-        // the async proxy refills the stage after this warp's own writes to it
-        if (wrote) fence_proxy_async_cta();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.empty[s]);
-
         if (d.w & TILE_LAST) {
             // ---- merge the warps' states in warp order; finish the run or leave its part
+            consumers_all(true);  // the stage has been read by all
+            float* acc = reinterpret_cast<float*>(kt);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     float l = l_run[nt][j];
@@ -392,161 +414,241 @@ __global__ void __launch_bounds__(kThreads, 2)
                         sm.l[warp][nt * 8 + 2 * t4 + j] = l;
                     }
                 }
-            if (!meet()) return;
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[(warp * C::kHeads + nt * 8 + 2 * t4 + (e & 1)) * kAccPitch + dt * 16 + g + (e >> 1) * 8] =
+                            o[nt][dt][e];
+            }
+            wrote = true;
+            consumers_all(true);
             const bool whole = (d.w & TILE_WHOLE) != 0;
-            const int part = b * 2 + ((d.w & TILE_BEGIN) ? 1 : 0);
-            if (tid < C::kHeads) {
-                float M = -INFINITY, L = 0.f;
-                for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.m[w][tid]);
+            const int part = (d.w >> 16) * 2 + ((d.w & TILE_BEGIN) ? 1 : 0);
+            // 64 pairs of dims by 2 heads at a time: thread tid has pair tid % 64 of head tid / 64 + 2 i
+            for (int h = tid >> 6; h < G; h += 2) {
+                float M = -INFINITY, L = 0.f, f[kWarps];
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.m[w][h]);
                 const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
-                    sm.f[w][tid] = exp2f(sm.m[w][tid] - base);
-                    L += sm.l[w][tid] * sm.f[w][tid];
+                    f[w] = exp2f(sm.m[w][h] - base);
+                    L += sm.l[w][h] * f[w];
                 }
-                if (poisoned) M = INFINITY, L = 0.f;  // no sum has this pair: an infinite score's sum is NaN
-                sm.cm[tid] = M;
-                sm.cl[tid] = L;
-                if (tid < G) {
-                    if (!whole)
-                        parts.pml[static_cast<size_t>(part) * parts.heads + tid] = make_float2(M, L);
-                    else if (a.accumulate)
-                        parts.ml[static_cast<size_t>(d.x) * a.q_heads + d.y * G + tid] = make_float2(M, L);
+                const float inv = poisoned ? 0.f : 1.f / L;
+                const int dd = (tid & 63) * 2;
+                float x = 0.f, y = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float2 v = *reinterpret_cast<const float2*>(&acc[(w * C::kHeads + h) * kAccPitch + dd]);
+                    x += v.x * f[w];
+                    y += v.y * f[w];
+                }
+                if (whole) {
+                    const float nan = __int_as_float(0x7FC00000);
+                    *reinterpret_cast<uint32_t*>(a.out + d.x * a.out_stride +
+                                                 (static_cast<size_t>(d.y) * G + h) * kCacheHd + dd) =
+                        poisoned ? pack_bf2(f2bf(nan), f2bf(nan)) : pack_bf2(f2bf(x * inv), f2bf(y * inv));
+                    if (dd == 0 && a.accumulate)
+                        parts.ml[static_cast<size_t>(d.x) * a.q_heads + d.y * G + h] = make_float2(base, inv);
+                } else {
+                    const size_t at = static_cast<size_t>(part) * G + h;
+                    *reinterpret_cast<float2*>(parts.po + at * kCacheHd + dd) = make_float2(x, y);
+                    // no other part has a poisoned one's pair: the sum to an infinite maximum is NaN
+                    if (dd == 0) parts.pml[at] = poisoned ? make_float2(INFINITY, 0.f) : make_float2(M, L);
                 }
             }
+        }
+        // the async proxy refills the stage after this warp's own writes to it
+        if (wrote) fence_proxy_async_cta();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.empty[s]);
+    }
+}
+
+// The second kernel: joins the parts of cut runs and turns scores into weights.  Its
+// warps take equal contiguous shares of the tiles, each on its own: a warp finds the
+// maximum and sum of every run it meets from that run's parts, writes the weights of
+// its slots, and joins an equal slice of the run's outputs (as many slices as warps
+// that meet the run).  Small enough to be resident beside two CTAs of the first
+// kernel: what depends on the lengths alone happens while that one runs.
+constexpr int kJoinThreads = 128;
+constexpr int kJoinWarps = kJoinThreads / 32;
+struct JoinSmem {
+    float2 ml[kJoinWarps][16];  // of the run at hand: maximum, 1 / sum (0: a bad page, no weights)
+    Plan plan;
+    int before[kJoinThreads + 1];
+    int scan[kJoinWarps];
+};
+
+// Weights of n slots from their scores: w[j] += sum_h 2^(s[j][h] - m_h) / l_h.  GV: the
+// heads (0: any number, in `heads`); U slots a lane in flight.
+template <int GV, int U>
+__device__ __forceinline__ void add_weights(float* w, const float* s, const float2* ml, int n, int heads, int lane) {
+    const int G = GV ? GV : heads;
+    for (int j0 = 0; j0 < n; j0 += 32 * U) {
+        float x[U], sc[U][GV ? GV : 1];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * 32 + lane;
+            x[u] = j < n ? w[j] : 0.f;
+            if constexpr (GV > 0) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            sm.acc[warp][nt * 8 + 2 * t4 + (e & 1)][dt * 16 + g + (e >> 1) * 8] = o[nt][half * 4 + dt][e];
-                if (!meet()) return;
-                for (int i = tid; i < G * 32; i += kConsumers) {
-                    const int h = i >> 5, dd = (i & 31) * 2;
-                    float x = 0.f, y = 0.f;
-#pragma unroll
-                    for (int w = 0; w < kWarps; ++w) {
-                        const float2 v = *reinterpret_cast<const float2*>(&sm.acc[w][h][dd]);
-                        x += v.x * sm.f[w][h];
-                        y += v.y * sm.f[w][h];
-                    }
-                    if (whole) {
-                        const float L = sm.cl[h];
-                        const bool nan = sm.cm[h] == INFINITY && L == 0.f;
-                        const bf16 u = f2bf(nan ? __int_as_float(0x7FC00000) : x / L);
-                        const bf16 v = f2bf(nan ? __int_as_float(0x7FC00000) : y / L);
-                        *reinterpret_cast<uint32_t*>(a.out + d.x * a.out_stride +
-                                                     (static_cast<size_t>(d.y) * G + h) * kCacheHd + half * 64 + dd) =
-                            pack_bf2(u, v);
+                for (int h = 0; h < GV; h += 4) {
+                    if constexpr (GV >= 4) {
+                        const float4 v = j < n ? *reinterpret_cast<const float4*>(s + static_cast<size_t>(j) * GV + h)
+                                               : make_float4(0.f, 0.f, 0.f, 0.f);
+                        sc[u][h] = v.x, sc[u][h + 1] = v.y, sc[u][h + 2] = v.z, sc[u][h + 3] = v.w;
+                    } else if constexpr (GV == 2) {
+                        const float2 v = j < n ? *reinterpret_cast<const float2*>(s + static_cast<size_t>(j) * 2)
+                                               : make_float2(0.f, 0.f);
+                        sc[u][0] = v.x, sc[u][1] = v.y;
                     } else {
-                        *reinterpret_cast<float2*>(parts.po + (static_cast<size_t>(part) * parts.heads + h) * kCacheHd +
-                                                   half * 64 + dd) = make_float2(x, y);
+                        sc[u][0] = j < n ? s[j] : 0.f;
                     }
                 }
-                if (!meet()) return;
             }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * 32 + lane;
+            float p = 0.f;
+            if constexpr (GV > 0) {
+#pragma unroll
+                for (int h = 0; h < GV; ++h) p += exp2f(sc[u][h] - ml[h].x) * ml[h].y;
+            } else if (j < n) {
+                for (int h = 0; h < G; ++h) p += exp2f(s[static_cast<size_t>(j) * G + h] - ml[h].x) * ml[h].y;
+            }
+            if (j < n) w[j] = x[u] + p;
         }
     }
 }
 
-// The second kernel, one CTA per share: joins the parts of cut runs (each of a run's
-// shares takes an equal slice of its outputs) and turns the share's scores into
-// weights (a warp per tile).
-struct JoinSmem {
-    float2 ml[2][16];  // of the share's parts, by slot: maximum, 1 / sum; 1 / sum = 0: a bad page, no weights
-    int chunk[kJoinThreads + 1];
-    int scan[kJoinThreads / 32];
-};
-
-__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(const __grid_constant__ CacheAttnArgs a, const Parts parts) {
+__global__ void __maxnreg__(64)
+    cache_join_kernel(const __grid_constant__ CacheAttnArgs a, const Parts parts) {
     __shared__ JoinSmem sm;
     const CacheView& c = a.c;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.q_heads / c.kv_heads;
-    scan_rows<kJoinThreads>(a.lens, c, sm.chunk, sm.scan);
-    const long long total = static_cast<long long>(sm.chunk[kJoinThreads]) * c.kv_heads;
-    const int shares = plan_shares(total, parts.shares);
-    const long long t0 = plan_first(total, shares, b);
-    const int n = b < shares ? static_cast<int>(plan_first(total, shares, b + 1) - t0) : 0;
+    scan_rows<kJoinThreads>(a.lens, c, sm.before, sm.scan);
+    const int total = sm.before[kJoinThreads] * c.kv_heads;
+    if (tid == 0) plan_make(sm.plan, total, parts.workers);
+    __syncthreads();
+    const Plan& plan = sm.plan;
+    // neighbouring shares on different SMs
+    const int shares = gridDim.x * kJoinWarps, me = warp * gridDim.x + blockIdx.x;
+    int t = equal_first(total, shares, me);
+    const int t1 = equal_first(total, shares, me + 1);
+    PlanPlace p;
+    int c0 = 0, c1 = 0;
+    auto enter_run = [&]() {  // the run of tile t
+        p = locate<kJoinThreads>(t, a.lens, c, sm.before);
+        c0 = plan_chunk_of(plan, t - p.tile);
+        c1 = plan_chunk_of(plan, t - p.tile + p.tiles - 1);
+    };
+    if (t < t1) enter_run();
     pdl_wait();
-    if (n == 0) return;
-    // ---- the share's first and last run, where they are cut
-    for (int e = 0; e < 2; ++e) {
-        const long long t = e == 0 ? t0 : t0 + n - 1;
-        const PlanPlace p = locate<kJoinThreads>(t, a.lens, c, sm.chunk);
-        const long long run0 = t - p.tile;
-        const int c0 = plan_share(total, shares, run0);
-        const int c1 = plan_share(total, shares, run0 + p.tiles - 1);
-        if (c0 == c1 || (e == 1 && run0 <= t0)) continue;  // whole, or the first run again
-        const int slot = plan_slot(total, shares, b, run0);
-        // the run begins in share c0: its part there is in slot 1, the others' in slot 0
-        auto part_of = [&](int share) { return static_cast<size_t>(share * 2 + (share == c0 ? 1 : 0)); };
-        for (int h = warp; h < G; h += kJoinThreads / 32) {
-            float M = -INFINITY;
+    if (me == 0 && lane == 0) *c.next_chunk = 0;  // for the cache's next attention
+    float2* ml = sm.ml[warp];
+    while (t < t1) {
+        const int run0 = t - p.tile, end = min(t1, run0 + p.tiles);
+        // the run begins in chunk c0: its part there is in slot 1, the others' in slot 0
+        auto part_of = [&](int chunk) { return static_cast<size_t>(chunk * 2 + (chunk == c0 ? 1 : 0)) * G; };
+        const bool cut = c0 != c1;
+        __syncwarp();
+        if (!cut) {
+            if (a.accumulate && lane < G) ml[lane] = parts.ml[static_cast<size_t>(p.row) * a.q_heads + p.head * G + lane];
+        } else {
+            // lane: head lane % wide of every (32 / wide)-th part, wide the power of two that holds G
+            const int wide = G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : G <= 8 ? 8 : 16;
+            const int h = lane % wide, deal = 32 / wide;
+            float M = -INFINITY, L = 0.f;
             bool bad = false;
-            for (int s = c0 + lane; s <= c1; s += 32) {
-                const float2 v = parts.pml[part_of(s) * parts.heads + h];
-                bad = bad || (v.x == INFINITY && v.y == 0.f);
-                M = fmaxf(M, v.x);
-            }
-            M = warp_max(M);
-            const float base = M == -INFINITY ? 0.f : M;
-            float L = 0.f;
-            for (int s = c0 + lane; s <= c1; s += 32) {
-                const float2 v = parts.pml[part_of(s) * parts.heads + h];
-                L += v.y * exp2f(v.x - base);
-            }
-            L = warp_sum(L);
-            bad = __any_sync(0xffffffffu, bad);
-            if (lane == 0) sm.ml[slot][h] = make_float2(base, bad ? 0.f : 1.f / L);
-        }
-        __syncthreads();
-        const int P = c1 - c0 + 1, outputs = G * kCacheHd;
-        const int o0 = static_cast<int>(static_cast<long long>(outputs) * (b - c0) / P);
-        const int o1 = static_cast<int>(static_cast<long long>(outputs) * (b - c0 + 1) / P);
-        for (int i = o0 + tid; i < o1; i += kJoinThreads) {
-            const int h = i / kCacheHd;
-            const float2 ml = sm.ml[slot][h];
-            float x = 0.f;
-            for (int s = c0; s <= c1; ++s) {
-                const size_t at = part_of(s) * parts.heads + h;
-                x += parts.po[at * kCacheHd + i % kCacheHd] * exp2f(parts.pml[at].x - ml.x);
-            }
-            a.out[p.row * a.out_stride + static_cast<size_t>(p.head) * outputs + i] =
-                f2bf(ml.y == 0.f ? __int_as_float(0x7FC00000) : x * ml.y);
-        }
-    }
-    if (!a.accumulate) return;
-    // ---- weights
-    for (int k = warp; k < n; k += kJoinThreads / 32) {
-        const long long t = t0 + k;
-        const PlanPlace p = locate<kJoinThreads>(t, a.lens, c, sm.chunk);
-        const long long run0 = t - p.tile;
-        const bool whole = run0 >= t0 && run0 + p.tiles <= t0 + n;
-        const int slot = run0 >= t0 ? 1 : 0;
-        const int valid = min(kCachePage, p.len - p.tile * kCachePage);
-        float* w = c.weights + cache_slot_index(c, p.row, p.head) + p.tile * kCachePage;
-        const float2* whole_ml = parts.ml + static_cast<size_t>(p.row) * a.q_heads + p.head * G;
-        for (int j = lane; j < valid; j += 32) {
-            const float* s = parts.score + (t * kCachePage + j) * G;
-            float sum = 0.f;
-            bool bad = false;
-            for (int h = 0; h < G; ++h) {
-                float2 ml;
-                if (whole) {
-                    ml = whole_ml[h];
-                    bad = bad || (ml.x == INFINITY && ml.y == 0.f);
-                    ml = make_float2(ml.x == -INFINITY ? 0.f : ml.x, 1.f / ml.y);
-                } else {
-                    ml = sm.ml[slot][h];
-                    bad = bad || ml.y == 0.f;
+            if (h < G)
+                for (int s0 = c0 + lane / wide; s0 <= c1; s0 += 4 * deal) {
+                    float2 v[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        v[u] = s0 + u * deal <= c1 ? parts.pml[part_of(s0 + u * deal) + h] : make_float2(-INFINITY, 0.f);
+                    float m = M;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        bad = bad || (v[u].x == INFINITY && v[u].y == 0.f);
+                        m = fmaxf(m, v[u].x);
+                    }
+                    const float base = m == -INFINITY ? 0.f : m;
+                    L *= exp2f(M - base);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) L += v[u].y * exp2f(v[u].x - base);
+                    M = m;
                 }
-                sum += exp2f(s[h] - ml.x) * ml.y;
+            for (int off = wide; off < 32; off <<= 1) {
+                const float m2 = __shfl_xor_sync(0xffffffffu, M, off), l2 = __shfl_xor_sync(0xffffffffu, L, off);
+                const float m = fmaxf(M, m2), base = m == -INFINITY ? 0.f : m;
+                // the same order of the two on both sides
+                const float x = L * exp2f(M - base), y = l2 * exp2f(m2 - base);
+                L = (lane & off) ? y + x : x + y;
+                M = m;
             }
-            if (!bad) w[j] += sum;
+            bad = __any_sync(0xffffffffu, bad);
+            if (lane < G) ml[lane] = make_float2(M == -INFINITY ? 0.f : M, bad ? 0.f : 1.f / L);
         }
+        __syncwarp();
+        if (cut) {
+            // outputs in units of 4 dims, lanes: unit lane % wide of every (32 / wide)-th part
+            const int first = equal_share_of(total, shares, run0);
+            const int slices = equal_share_of(total, shares, run0 + p.tiles - 1) - first + 1, units = G * kCacheHd / 4;
+            const int u0 = equal_first(units, slices, me - first), u1 = equal_first(units, slices, me - first + 1);
+            int wide = 1;
+            while (wide < u1 - u0 && wide < 32) wide *= 2;
+            const int deal = 32 / wide;
+            for (int u = u0; u < u1; u += wide) {
+                const int mine = u + lane % wide;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                const int h = min(mine, u1 - 1) / (kCacheHd / 4);
+                const float base = ml[h].x, inv = ml[h].y;
+                if (mine < u1)
+#pragma unroll 4
+                    for (int s = c0 + lane / wide; s <= c1; s += deal) {
+                        const size_t at = part_of(s) + h;
+                        const float f = exp2f(parts.pml[at].x - base);
+                        const float4 v = reinterpret_cast<const float4*>(parts.po + at * kCacheHd)[mine % (kCacheHd / 4)];
+                        x.x += v.x * f, x.y += v.y * f, x.z += v.z * f, x.w += v.w * f;
+                    }
+                for (int off = wide; off < 32; off <<= 1) {
+                    x.x += __shfl_xor_sync(0xffffffffu, x.x, off);
+                    x.y += __shfl_xor_sync(0xffffffffu, x.y, off);
+                    x.z += __shfl_xor_sync(0xffffffffu, x.z, off);
+                    x.w += __shfl_xor_sync(0xffffffffu, x.w, off);
+                }
+                if (lane < wide && mine < u1) {
+                    if (inv == 0.f) x = make_float4(NAN, NAN, NAN, NAN);
+                    const float k = inv == 0.f ? 1.f : inv;
+                    uint2 o;
+                    o.x = pack_bf2(f2bf(x.x * k), f2bf(x.y * k));
+                    o.y = pack_bf2(f2bf(x.z * k), f2bf(x.w * k));
+                    reinterpret_cast<uint2*>(a.out + p.row * a.out_stride + static_cast<size_t>(p.head) * G * kCacheHd)[mine] = o;
+                }
+            }
+        }
+        if (a.accumulate) {
+            bool bad = false;
+            for (int h = 0; h < G; ++h) bad = bad || ml[h].y == 0.f;
+            const int n = min((end - t) * kCachePage, p.len - p.tile * kCachePage);
+            float* w = c.weights + cache_slot_index(c, p.row, p.head) + p.tile * kCachePage;
+            const float* s = parts.score + static_cast<size_t>(t) * kCachePage * G;
+            if (!bad) switch (G) {
+                    case 1: add_weights<1, 8>(w, s, ml, n, G, lane); break;
+                    case 2: add_weights<2, 8>(w, s, ml, n, G, lane); break;
+                    case 4: add_weights<4, 4>(w, s, ml, n, G, lane); break;
+                    case 8: add_weights<8, 4>(w, s, ml, n, G, lane); break;
+                    case 16: add_weights<16, 2>(w, s, ml, n, G, lane); break;
+                    default: add_weights<0, 2>(w, s, ml, n, G, lane);
+                }
+        }
+        t = end;
+        if (t < t1) enter_run();
     }
 }
 
@@ -569,24 +671,25 @@ size_t max_tiles(const CacheView& c) {
 }
 
 // Two resident CTAs an SM, no more than there can be tiles.
-int shares_of(const CacheView& c, int sms) {
+int workers_of(const CacheView& c, int sms) {
     return static_cast<int>(std::min(static_cast<size_t>(2 * sms), max_tiles(c)));
 }
 
 // The workspace's arrays from its start; returns its size.
 size_t layout(const CacheView& c, int q_heads, int accumulate, int sms, uint8_t* ws, Parts* p) {
-    const int G = q_heads / c.kv_heads, shares = shares_of(c, sms);
+    const int G = q_heads / c.kv_heads, workers = workers_of(c, sms);
+    const size_t parts = 2 * static_cast<size_t>(plan_most_chunks(static_cast<int>(max_tiles(c)), workers));
     size_t at = 0;
     auto take = [&](size_t bytes) {
         uint8_t* to = ws + at;
         at += pad256(bytes);
         return to;
     };
-    p->shares = shares;
+    p->workers = workers;
     p->heads = G;
     p->ml = reinterpret_cast<float2*>(take(static_cast<size_t>(c.rows) * q_heads * 8));
-    p->pml = reinterpret_cast<float2*>(take(static_cast<size_t>(shares) * 2 * G * 8));
-    p->po = reinterpret_cast<float*>(take(static_cast<size_t>(shares) * 2 * G * kCacheHd * 4));
+    p->pml = reinterpret_cast<float2*>(take(parts * G * 8));
+    p->po = reinterpret_cast<float*>(take(parts * G * kCacheHd * 4));
     p->score = reinterpret_cast<float*>(take(accumulate ? max_tiles(c) * kCachePage * G * 4 : 0));
     return at;
 }
@@ -608,7 +711,7 @@ cudaError_t launch_nt(const CacheAttnArgs& a, const Maps& maps, const Parts& par
         if (e != cudaSuccess) return e;
         configured.fetch_or(bit);
     }
-    cache_attention_kernel<NT><<<parts.shares, kThreads, sizeof(Smem<NT>) + 1024, s>>>(a, maps, parts);
+    cache_attention_kernel<NT><<<parts.workers, kThreads, sizeof(Smem<NT>) + 1024, s>>>(a, maps, parts);
     return cudaGetLastError();
 }
 
@@ -631,7 +734,7 @@ cudaError_t launch_cache_attention(const CacheAttnArgs& a, int sms, cudaStream_t
     cudaError_t e = a.q_heads / c.kv_heads <= 8 ? launch_nt<1>(a, maps, parts, s) : launch_nt<2>(a, maps, parts, s);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(parts.shares);
+    cfg.gridDim = dim3(parts.workers);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];

@@ -1,5 +1,6 @@
 // Checks the work shares of the attention over a bounded paged cache
 // (csrc/cache_plan.hpp) against a brute-force walk; run by test_cache.py.
+#include <climits>
 #include <cstdio>
 #include <cstdlib>
 #include <random>
@@ -19,53 +20,80 @@ using namespace q3;
         }                                                      \
     } while (0)
 
-static void check(const std::vector<int32_t>& lens, int kvh, int max_len, int most, int chunks) {
+static void check_totals(int total, int workers) {
+    Plan p;
+    plan_make(p, total, workers);
+    REQUIRE(p.tiers <= kPlanTiers && p.chunks <= plan_most_chunks(total, workers));
+    REQUIRE(p.tile0[p.tiers] == total && p.chunk0[p.tiers] == p.chunks);
+    REQUIRE(plan_most_chunks(total, workers) <= plan_most_chunks(total < INT_MAX - 5 ? total + 5 : total, workers));
+    int first = 0, end = 0, at = 0;
+    const int step = p.chunks > 5000 ? 37 : 1;
+    for (int c = 0; c < p.chunks; c += step) {
+        plan_chunk(p, c, first, end);
+        REQUIRE(first < end && end <= total);
+        if (step == 1) {
+            REQUIRE(first == at);
+            at = end;
+        }
+        REQUIRE(plan_chunk_of(p, first) == c && plan_chunk_of(p, end - 1) == c);
+    }
+    if (total > 0) {
+        plan_chunk(p, p.chunks - 1, first, end);
+        REQUIRE(end == total);
+    }
+    for (const int parts : {1, 7, workers, 4 * workers}) {
+        REQUIRE(equal_first(total, parts, 0) == 0 && equal_first(total, parts, parts) == total);
+        for (int i = 0; i < parts; ++i) {
+            const int a = equal_first(total, parts, i), b = equal_first(total, parts, i + 1);
+            REQUIRE(a <= b);
+            if (a < b) REQUIRE(equal_share_of(total, parts, a) == i && equal_share_of(total, parts, b - 1) == i);
+        }
+    }
+}
+
+static void check(const std::vector<int32_t>& lens, int kvh, int max_len, int workers, int groups) {
     const int rows = static_cast<int>(lens.size());
     struct T {
-        int row, head, tile, tiles;
-        long long run0;
+        int row, head, tile, tiles, run0;
     };
     std::vector<T> all;
     for (int r = 0; r < rows; ++r) {
         const int n = lens[r] > 0 && lens[r] <= max_len ? (lens[r] + 63) / 64 : 0;
         REQUIRE(plan_tiles(lens[r], max_len) == n);
         for (int h = 0; h < kvh; ++h) {
-            const long long run0 = static_cast<long long>(all.size());
+            const int run0 = static_cast<int>(all.size());
             for (int i = 0; i < n; ++i) all.push_back({r, h, i, n, run0});
         }
     }
-    const long long total = static_cast<long long>(all.size());
-    if (total == 0) return;
-    std::vector<int> chunk(chunks + 1, 0);
-    const int per = plan_chunk_rows(rows, chunks);
-    for (int i = 0; i < chunks; ++i) {
-        chunk[i + 1] = chunk[i];
-        for (int r = i * per; r < rows && r < (i + 1) * per; ++r) chunk[i + 1] += plan_tiles(lens[r], max_len);
+    const int total = static_cast<int>(all.size());
+    check_totals(total, workers);
+    Plan plan;
+    plan_make(plan, total, workers);
+    std::vector<int> before(groups + 1, 0);
+    const int per = plan_group_rows(rows, groups);
+    for (int i = 0; i < groups; ++i) {
+        before[i + 1] = before[i];
+        for (int r = i * per; r < rows && r < (i + 1) * per; ++r) before[i + 1] += plan_tiles(lens[r], max_len);
     }
-    REQUIRE(static_cast<long long>(chunk[chunks]) * kvh == total);
-    const int shares = plan_shares(total, most);
-    REQUIRE(shares >= 1 && shares <= most);
-    REQUIRE(plan_first(total, shares, 0) == 0 && plan_first(total, shares, shares) == total);
+    REQUIRE(before[groups] * kvh == total);
     std::set<std::pair<int, int>> used;
-    for (int b = 0; b < shares; ++b) {
-        const long long t0 = plan_first(total, shares, b), t1 = plan_first(total, shares, b + 1);
-        REQUIRE(t1 > t0 && t1 - t0 >= total / shares && t1 - t0 <= total / shares + 1);
-        for (long long t = t0; t < t1; ++t) {
-            REQUIRE(plan_share(total, shares, t) == b);
-            const PlanPlace p = plan_locate(t, lens.data(), rows, max_len, kvh, chunk.data(), chunks);
+    for (int c = 0; c < plan.chunks; ++c) {
+        int t0 = 0, t1 = 0;
+        plan_chunk(plan, c, t0, t1);
+        for (int t = t0; t < t1; ++t) {
+            const PlanPlace p = plan_locate(t, lens.data(), rows, max_len, kvh, before.data(), groups);
             const T& w = all[t];
             REQUIRE(p.row == w.row && p.head == w.head && p.tile == w.tile && p.tiles == w.tiles &&
                     p.len == lens[w.row]);
             const bool first = t == t0 || w.tile == 0;
             const bool whole = w.run0 >= t0 && w.run0 + w.tiles <= t1;
-            if (first && !whole) {  // a part: its slot is its own
-                const int slot = plan_slot(total, shares, b, w.run0);
-                REQUIRE(slot == (w.run0 >= t0 ? 1 : 0));
-                REQUIRE(used.insert({b, slot}).second);
-                // found again from the run alone: the first share in its slot, the others in slot 0
-                const int c0 = plan_share(total, shares, w.run0);
-                REQUIRE(c0 <= b && b <= plan_share(total, shares, w.run0 + w.tiles - 1));
-                REQUIRE(b == c0 ? slot == 1 : slot == 0);
+            const int c0 = plan_chunk_of(plan, w.run0), c1 = plan_chunk_of(plan, w.run0 + w.tiles - 1);
+            REQUIRE((c0 == c1) == whole);
+            if (first && !whole) {  // a part: its slot is its own, and follows from the run's first chunk
+                const int slot = w.run0 >= t0 ? 1 : 0;
+                REQUIRE(used.insert({c, slot}).second);
+                REQUIRE(c0 <= c && c <= c1);
+                REQUIRE((c == c0) == (slot == 1));
             }
         }
     }
@@ -86,8 +114,10 @@ int main() {
     check(std::vector<int32_t>(4096, 1), 1, 1, 296, 160);
     check(std::vector<int32_t>(4096, 65), 2, 130, 296, 512);
     check({1000000}, 3, 1 << 20, 296, 160);
-    // the largest total stays inside 64 bits
-    const long long most = 4096ll * 1024 * 16384;
-    REQUIRE(plan_share(most, 296, most - 1) == 295 && plan_first(most, 296, 296) == most);
+    check({0, -1, 500}, 3, 100, 296, 160);
+    for (int t = 0; t < 3000; ++t) check_totals(t, pick(1, 400));
+    for (const int workers : {1, 2, 147, 296, 1000})
+        for (const int t : {7 * workers, 8 * workers - 1, 8 * workers, 8 * workers + 1, 1000 * workers + 5, 1 << 24, INT_MAX})
+            if (t / workers < 1 << 24 || workers > 100) check_totals(t, workers);
     std::puts("ok");
 }

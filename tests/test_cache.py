@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 
 GOOD = dict(k_pages=4096, v_pages=8192, num_pages=10, page_tables=64, table_stride=2, weights=128, positions=256,
-            slot_stride=128, rows=4, max_len=128, kv_heads=2, head_dim=128, page_size=64, error=32)
+            slot_stride=128, rows=4, max_len=128, kv_heads=2, head_dim=128, page_size=64, state=32)
 
 
 def create(**change):
@@ -28,8 +28,8 @@ def cache():
 
 
 @pytest.mark.parametrize("change,status", [
-    (dict(k_pages=None), 1), (dict(v_pages=None), 1), (dict(page_tables=None), 1), (dict(error=None), 1),
-    (dict(k_pages=4104), 1), (dict(page_tables=66), 1), (dict(weights=130), 1), (dict(error=34), 1),
+    (dict(k_pages=None), 1), (dict(v_pages=None), 1), (dict(page_tables=None), 1), (dict(state=None), 1),
+    (dict(k_pages=4104), 1), (dict(page_tables=66), 1), (dict(weights=130), 1), (dict(state=34), 1),
     (dict(weights=None), 1), (dict(positions=None), 1), (dict(head_dim=64), 3), (dict(page_size=16), 3),
     (dict(kv_heads=0), 1), (dict(rows=0), 1), (dict(rows=4097), 1), (dict(max_len=0), 1),
     (dict(max_len=(1 << 20) + 1), 1), (dict(max_len=129), 1), (dict(slot_stride=127), 1), (dict(num_pages=0), 1),
