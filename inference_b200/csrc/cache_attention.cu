@@ -63,9 +63,8 @@ struct Smem {
     // stage is where the warps' outputs meet ([warp][head][kAccPitch] floats)
     uint8_t ring[Cfg<NT>::kStages][Cfg<NT>::kStageBytes];
     float m[kWarps][Cfg<NT>::kHeads], l[kWarps][Cfg<NT>::kHeads];
-    int4 tile[Cfg<NT>::kStages];        // row, head, tile, flags | live slots << 8 | chunk << 16
+    int4 tile[Cfg<NT>::kStages];        // row, head, tile, flags | live slots << 8 | chunk's place << 16
     uint64_t full[Cfg<NT>::kStages], empty[Cfg<NT>::kStages];
-    Plan plan;
     int before[kThreads + 1];           // tiles before each group of rows
     int scan[kThreads / 32];
 };
@@ -164,9 +163,7 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
 
     if (warp == kWarps) {
         // ------------------------------------------------------------ producer
-        if (lane == 0) plan_make(sm.plan, sm.before[kThreads] * c.kv_heads, parts.workers);
-        __syncwarp();
-        const Plan& plan = sm.plan;
+        const Plan plan = plan_make(sm.before[kThreads] * c.kv_heads, parts.workers);
         const uint64_t pol = policy_evict_first();
         int k = 0;        // tiles issued
         bool ok = true;
@@ -180,8 +177,8 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
             // the chunk after this one, asked for ahead: whoever is free first takes the next
             int next = plan.chunks;
             if (lane == 0 && plan.chunks > gridDim.x) next = gridDim.x + static_cast<int>(atomicAdd(c.next_chunk, 1u));
-            int t0, t1;
-            plan_chunk(plan, chunk, t0, t1);
+            int t0, t1, place;
+            plan_chunk(plan, chunk, t0, t1, place);
             for (int i0 = t0; i0 < t1 && ok; i0 += 32) {
                 // lane i: tile i0 + i
                 int4 d = make_int4(0, 0, 0, 0);
@@ -203,7 +200,7 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                     } else {
                         y = (page * c.kv_heads + p.head) * kCachePage;
                     }
-                    d = make_int4(p.row, p.head, t, flags | min(kCachePage, p.len - p.tile * kCachePage) << 8 | chunk << 16);
+                    d = make_int4(p.row, p.head, t, flags | min(kCachePage, p.len - p.tile * kCachePage) << 8 | place << 16);
                 }
                 for (int i = 0; i < 32 && i0 + i < t1 && ok; ++i, ++k) {
                     const int4 t = make_int4(__shfl_sync(0xffffffffu, d.x, i), __shfl_sync(0xffffffffu, d.y, i),
@@ -475,9 +472,9 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
 // kernel: what depends on the lengths alone happens while that one runs.
 constexpr int kJoinThreads = 128;
 constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinCtas = 8;  // an SM
 struct JoinSmem {
     float2 ml[kJoinWarps][16];  // of the run at hand: maximum, 1 / sum (0: a bad page, no weights)
-    Plan plan;
     int before[kJoinThreads + 1];
     int scan[kJoinWarps];
 };
@@ -533,19 +530,18 @@ __global__ void __maxnreg__(64)
     const int G = a.q_heads / c.kv_heads;
     scan_rows<kJoinThreads>(a.lens, c, sm.before, sm.scan);
     const int total = sm.before[kJoinThreads] * c.kv_heads;
-    if (tid == 0) plan_make(sm.plan, total, parts.workers);
-    __syncthreads();
-    const Plan& plan = sm.plan;
+    const Plan plan = plan_make(total, parts.workers);
     // neighbouring shares on different SMs
     const int shares = gridDim.x * kJoinWarps, me = warp * gridDim.x + blockIdx.x;
-    int t = equal_first(total, shares, me);
-    const int t1 = equal_first(total, shares, me + 1);
+    const Equal mine = equal_make(total, shares);
+    int t = equal_first(mine, me);
+    const int t1 = equal_first(mine, me + 1);
     PlanPlace p;
     int c0 = 0, c1 = 0;
     auto enter_run = [&]() {  // the run of tile t
         p = locate<kJoinThreads>(t, a.lens, c, sm.before);
-        c0 = plan_chunk_of(plan, t - p.tile);
-        c1 = plan_chunk_of(plan, t - p.tile + p.tiles - 1);
+        c0 = plan_place_of(plan, t - p.tile);
+        c1 = plan_place_of(plan, t - p.tile + p.tiles - 1);
     };
     if (t < t1) enter_run();
     pdl_wait();
@@ -597,23 +593,23 @@ __global__ void __maxnreg__(64)
         __syncwarp();
         if (cut) {
             // outputs in units of 4 dims, lanes: unit lane % wide of every (32 / wide)-th part
-            const int first = equal_share_of(total, shares, run0);
-            const int slices = equal_share_of(total, shares, run0 + p.tiles - 1) - first + 1, units = G * kCacheHd / 4;
-            const int u0 = equal_first(units, slices, me - first), u1 = equal_first(units, slices, me - first + 1);
+            const int first = equal_share_of(mine, run0), units = G * kCacheHd / 4;
+            const Equal slice = equal_make(units, equal_share_of(mine, run0 + p.tiles - 1) - first + 1);
+            const int u0 = equal_first(slice, me - first), u1 = equal_first(slice, me - first + 1);
             int wide = 1;
             while (wide < u1 - u0 && wide < 32) wide *= 2;
             const int deal = 32 / wide;
             for (int u = u0; u < u1; u += wide) {
-                const int mine = u + lane % wide;
+                const int unit = u + lane % wide;
                 float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                const int h = min(mine, u1 - 1) / (kCacheHd / 4);
+                const int h = min(unit, u1 - 1) / (kCacheHd / 4);
                 const float base = ml[h].x, inv = ml[h].y;
-                if (mine < u1)
+                if (unit < u1)
 #pragma unroll 4
                     for (int s = c0 + lane / wide; s <= c1; s += deal) {
                         const size_t at = part_of(s) + h;
                         const float f = exp2f(parts.pml[at].x - base);
-                        const float4 v = reinterpret_cast<const float4*>(parts.po + at * kCacheHd)[mine % (kCacheHd / 4)];
+                        const float4 v = reinterpret_cast<const float4*>(parts.po + at * kCacheHd)[unit % (kCacheHd / 4)];
                         x.x += v.x * f, x.y += v.y * f, x.z += v.z * f, x.w += v.w * f;
                     }
                 for (int off = wide; off < 32; off <<= 1) {
@@ -622,13 +618,13 @@ __global__ void __maxnreg__(64)
                     x.z += __shfl_xor_sync(0xffffffffu, x.z, off);
                     x.w += __shfl_xor_sync(0xffffffffu, x.w, off);
                 }
-                if (lane < wide && mine < u1) {
+                if (lane < wide && unit < u1) {
                     if (inv == 0.f) x = make_float4(NAN, NAN, NAN, NAN);
                     const float k = inv == 0.f ? 1.f : inv;
                     uint2 o;
                     o.x = pack_bf2(f2bf(x.x * k), f2bf(x.y * k));
                     o.y = pack_bf2(f2bf(x.z * k), f2bf(x.w * k));
-                    reinterpret_cast<uint2*>(a.out + p.row * a.out_stride + static_cast<size_t>(p.head) * G * kCacheHd)[mine] = o;
+                    reinterpret_cast<uint2*>(a.out + p.row * a.out_stride + static_cast<size_t>(p.head) * G * kCacheHd)[unit] = o;
                 }
             }
         }
@@ -678,7 +674,7 @@ int workers_of(const CacheView& c, int sms) {
 // The workspace's arrays from its start; returns its size.
 size_t layout(const CacheView& c, int q_heads, int accumulate, int sms, uint8_t* ws, Parts* p) {
     const int G = q_heads / c.kv_heads, workers = workers_of(c, sms);
-    const size_t parts = 2 * static_cast<size_t>(plan_most_chunks(static_cast<int>(max_tiles(c)), workers));
+    const size_t parts = 2 * static_cast<size_t>(workers) * plan_make(static_cast<int>(max_tiles(c)), workers).tiers;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         uint8_t* to = ws + at;
@@ -734,7 +730,7 @@ cudaError_t launch_cache_attention(const CacheAttnArgs& a, int sms, cudaStream_t
     cudaError_t e = a.q_heads / c.kv_heads <= 8 ? launch_nt<1>(a, maps, parts, s) : launch_nt<2>(a, maps, parts, s);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(parts.workers);
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min(static_cast<size_t>(kJoinCtas * sms), (max_tiles(c) + kJoinWarps - 1) / kJoinWarps)));
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];

@@ -21,81 +21,71 @@
 namespace q3 {
 
 constexpr int kPlanTile = 64;
-constexpr int kPlanTiers = 34;   // halvings of a 31-bit number, and the ends
-constexpr int kPlanSmall = 3;    // tiles of the last tier's chunks
+constexpr int kPlanSmall = 3;  // no chunk but a region's last is smaller than this many tiles
 
 Q3_HD int plan_tiles(int len, int max_len) {
     return len > 0 && len <= max_len ? (len + kPlanTile - 1) / kPlanTile : 0;
 }
 
-// Tiers of equal chunks.  With fewer than 8 tiles a worker: one chunk each, sizes
-// differing by one tile.  Otherwise 5/8 of the tiles as one chunk each, which the
-// workers begin with; the rest is taken as workers become free, every further tier
-// half of what is left, down to chunks of 3 tiles: SMs differ in the bandwidth they
-// get (on a B200, equal shares of 125 tiles took 157 to 204 us), and what a worker
-// finishes late is then at most a small chunk.
-struct Plan {
-    int total, tiers, chunks;
-    int tile0[kPlanTiers + 1], chunk0[kPlanTiers + 1], size[kPlanTiers];
-};
-Q3_HD void plan_add(Plan& p, int size, int count) {
-    if (size <= 0 || count <= 0) return;
-    p.size[p.tiers] = size;
-    ++p.tiers;
-    const long long end = static_cast<long long>(size) * count + p.tile0[p.tiers - 1];
-    p.tile0[p.tiers] = end < p.total ? static_cast<int>(end) : p.total;
-    p.chunks += count;
-    p.chunk0[p.tiers] = p.chunks;
-}
-Q3_HD void plan_make(Plan& p, int total, int workers) {
-    p.total = total;
-    p.tiers = p.chunks = 0;
-    p.tile0[0] = p.chunk0[0] = 0;
-    const int base = total / workers;
-    if (base < 8) {
-        plan_add(p, base + 1, total - base * workers);
-        plan_add(p, base, workers - (total - base * workers));
-        return;
-    }
-    int left = total;
-    int size = static_cast<int>(static_cast<long long>(base) * 5 / 8);
-    while (size >= kPlanSmall) {
-        plan_add(p, size, workers);
-        left -= size * workers;
-        size = left / (2 * workers);
-    }
-    plan_add(p, kPlanSmall, (left + kPlanSmall - 1) / kPlanSmall);
-}
-// No plan of at most `total` tiles has more chunks than this.
-Q3_HD int plan_most_chunks(int total, int workers) {
-    if (total < workers) return total < 1 ? 1 : total;
-    int tiers = 3;  // the first, and less than 2 chunks of 3 tiles a worker left for the last, and one
-    for (int base = total / workers; base >= 8; base /= 2) ++tiers;
-    return tiers * workers;
-}
-// Tiles [first, end) of chunk c.
-Q3_HD void plan_chunk(const Plan& p, int c, int& first, int& end) {
-    int k = 0;
-    while (k + 1 < p.tiers && p.chunk0[k + 1] <= c) ++k;
-    first = p.tile0[k] + (c - p.chunk0[k]) * p.size[k];
-    end = p.tile0[k + 1] - first > p.size[k] ? first + p.size[k] : p.tile0[k + 1];
-}
-// The chunk that holds tile t.
-Q3_HD int plan_chunk_of(const Plan& p, int t) {
-    int k = 0;
-    while (k + 1 < p.tiers && p.tile0[k + 1] <= t) ++k;
-    return p.chunk0[k] + (t - p.tile0[k]) / p.size[k];
-}
-
 // `total` tiles in `parts` equal shares (sizes differ by one): the first tile of share
 // i, and the share that holds tile t.
-Q3_HD int equal_first(int total, int parts, int i) {
-    const int base = total / parts, extra = total - base * parts;
-    return i * base + (i < extra ? i : extra);
+struct Equal {
+    int base, extra;
+};
+Q3_HD Equal equal_make(int total, int parts) {
+    Equal e;
+    e.base = total / parts;
+    e.extra = total - e.base * parts;
+    return e;
 }
-Q3_HD int equal_share_of(int total, int parts, int t) {
-    const int base = total / parts, extra = total - base * parts, big = extra * (base + 1);
-    return t < big ? t / (base + 1) : extra + (t - big) / base;
+Q3_HD int equal_first(const Equal& e, int i) { return i * e.base + (i < e.extra ? i : e.extra); }
+Q3_HD int equal_share_of(const Equal& e, int t) {
+    const int big = e.extra * (e.base + 1);
+    return t < big ? t / (e.base + 1) : e.extra + (t - big) / e.base;
+}
+
+// Every worker (CTA) has an equal region of the tiles.  Its first 5/8 are one chunk,
+// which it begins with; the rest is cut into chunks that halve down to 3 tiles and
+// are taken by whichever worker is free, the larger ones of all regions first: SMs
+// differ in the bandwidth they get (on a B200, whole regions of 125 tiles took 157 to
+// 204 us), and what a worker finishes late is at most a small chunk.  Regions below 8
+// tiles stay whole.  Chunk id = tier * workers + region gives the order of taking;
+// the order along the tiles is region * tiers + tier.
+Q3_HD int plan_rest(int base) { return base / 8 * 3 + base % 8 * 3 / 8; }
+struct Plan {
+    Equal region;
+    int workers, tiers, chunks;
+};
+Q3_HD Plan plan_make(int total, int workers) {
+    Plan p;
+    p.region = equal_make(total, workers);
+    p.workers = workers;
+    p.tiers = 1;
+    if (p.region.base >= 8)
+        for (int left = plan_rest(p.region.base); left >= kPlanSmall; left /= 2) ++p.tiers;
+    p.chunks = p.region.base > 0 ? p.tiers * workers : p.region.extra;
+    return p;
+}
+// The first tile of a tier in its region.
+Q3_HD int plan_tier(const Plan& p, int tier) {
+    if (tier == 0) return 0;
+    return p.region.base - (plan_rest(p.region.base) >> (tier - 1));
+}
+// Tiles [first, end) of chunk `id`, and its place along the tiles.
+Q3_HD void plan_chunk(const Plan& p, int id, int& first, int& end, int& place) {
+    int tier = 0, region = id;
+    while (region >= p.workers) region -= p.workers, ++tier;
+    const int begin = equal_first(p.region, region);
+    first = begin + plan_tier(p, tier);
+    end = tier + 1 < p.tiers ? begin + plan_tier(p, tier + 1) : equal_first(p.region, region + 1);
+    place = region * p.tiers + tier;
+}
+// The place of the chunk that holds tile t.
+Q3_HD int plan_place_of(const Plan& p, int t) {
+    const int region = equal_share_of(p.region, t), at = t - equal_first(p.region, region);
+    int tier = 0;
+    while (tier + 1 < p.tiers && plan_tier(p, tier + 1) <= at) ++tier;
+    return region * p.tiers + tier;
 }
 
 // Rows are scanned in `groups` groups of consecutive rows; before[i] = tiles of one

@@ -21,32 +21,33 @@ using namespace q3;
     } while (0)
 
 static void check_totals(int total, int workers) {
-    Plan p;
-    plan_make(p, total, workers);
-    REQUIRE(p.tiers <= kPlanTiers && p.chunks <= plan_most_chunks(total, workers));
-    REQUIRE(p.tile0[p.tiers] == total && p.chunk0[p.tiers] == p.chunks);
-    REQUIRE(plan_most_chunks(total, workers) <= plan_most_chunks(total < INT_MAX - 5 ? total + 5 : total, workers));
-    int first = 0, end = 0, at = 0;
-    const int step = p.chunks > 5000 ? 37 : 1;
-    for (int c = 0; c < p.chunks; c += step) {
-        plan_chunk(p, c, first, end);
-        REQUIRE(first < end && end <= total);
-        if (step == 1) {
-            REQUIRE(first == at);
-            at = end;
+    const Plan p = plan_make(total, workers);
+    REQUIRE(p.tiers >= 1 && p.tiers <= 31 && p.chunks <= p.tiers * workers);
+    REQUIRE(plan_make(total < INT_MAX - 5 ? total + 5 : total, workers).tiers >= p.tiers);  // the workspace's bound
+    std::vector<std::pair<int, int>> at(static_cast<size_t>(p.tiers) * workers, {-1, -1});
+    for (int id = 0; id < p.chunks; ++id) {
+        int first = 0, end = 0, place = 0;
+        plan_chunk(p, id, first, end, place);
+        REQUIRE(first < end && end <= total && place >= 0 && place < p.tiers * workers);
+        REQUIRE(at[place].first < 0);
+        at[place] = {first, end};
+        REQUIRE(plan_place_of(p, first) == place && plan_place_of(p, end - 1) == place);
+        REQUIRE(p.region.base < 8 || end - first >= kPlanSmall);
+    }
+    int next = 0;
+    for (const auto& c : at)
+        if (c.first >= 0) {
+            REQUIRE(c.first == next);
+            next = c.second;
         }
-        REQUIRE(plan_chunk_of(p, first) == c && plan_chunk_of(p, end - 1) == c);
-    }
-    if (total > 0) {
-        plan_chunk(p, p.chunks - 1, first, end);
-        REQUIRE(end == total);
-    }
+    REQUIRE(next == total);
     for (const int parts : {1, 7, workers, 4 * workers}) {
-        REQUIRE(equal_first(total, parts, 0) == 0 && equal_first(total, parts, parts) == total);
+        const Equal e = equal_make(total, parts);
+        REQUIRE(equal_first(e, 0) == 0 && equal_first(e, parts) == total);
         for (int i = 0; i < parts; ++i) {
-            const int a = equal_first(total, parts, i), b = equal_first(total, parts, i + 1);
+            const int a = equal_first(e, i), b = equal_first(e, i + 1);
             REQUIRE(a <= b);
-            if (a < b) REQUIRE(equal_share_of(total, parts, a) == i && equal_share_of(total, parts, b - 1) == i);
+            if (a < b) REQUIRE(equal_share_of(e, a) == i && equal_share_of(e, b - 1) == i);
         }
     }
 }
@@ -67,8 +68,7 @@ static void check(const std::vector<int32_t>& lens, int kvh, int max_len, int wo
     }
     const int total = static_cast<int>(all.size());
     check_totals(total, workers);
-    Plan plan;
-    plan_make(plan, total, workers);
+    const Plan plan = plan_make(total, workers);
     std::vector<int> before(groups + 1, 0);
     const int per = plan_group_rows(rows, groups);
     for (int i = 0; i < groups; ++i) {
@@ -78,8 +78,8 @@ static void check(const std::vector<int32_t>& lens, int kvh, int max_len, int wo
     REQUIRE(before[groups] * kvh == total);
     std::set<std::pair<int, int>> used;
     for (int c = 0; c < plan.chunks; ++c) {
-        int t0 = 0, t1 = 0;
-        plan_chunk(plan, c, t0, t1);
+        int t0 = 0, t1 = 0, place = 0;
+        plan_chunk(plan, c, t0, t1, place);
         for (int t = t0; t < t1; ++t) {
             const PlanPlace p = plan_locate(t, lens.data(), rows, max_len, kvh, before.data(), groups);
             const T& w = all[t];
@@ -87,13 +87,13 @@ static void check(const std::vector<int32_t>& lens, int kvh, int max_len, int wo
                     p.len == lens[w.row]);
             const bool first = t == t0 || w.tile == 0;
             const bool whole = w.run0 >= t0 && w.run0 + w.tiles <= t1;
-            const int c0 = plan_chunk_of(plan, w.run0), c1 = plan_chunk_of(plan, w.run0 + w.tiles - 1);
+            const int c0 = plan_place_of(plan, w.run0), c1 = plan_place_of(plan, w.run0 + w.tiles - 1);
             REQUIRE((c0 == c1) == whole);
             if (first && !whole) {  // a part: its slot is its own, and follows from the run's first chunk
                 const int slot = w.run0 >= t0 ? 1 : 0;
-                REQUIRE(used.insert({c, slot}).second);
-                REQUIRE(c0 <= c && c <= c1);
-                REQUIRE((c == c0) == (slot == 1));
+                REQUIRE(used.insert({place, slot}).second);
+                REQUIRE(c0 <= place && place <= c1);
+                REQUIRE((place == c0) == (slot == 1));
             }
         }
     }
@@ -118,6 +118,6 @@ int main() {
     for (int t = 0; t < 3000; ++t) check_totals(t, pick(1, 400));
     for (const int workers : {1, 2, 147, 296, 1000})
         for (const int t : {7 * workers, 8 * workers - 1, 8 * workers, 8 * workers + 1, 1000 * workers + 5, 1 << 24, INT_MAX})
-            if (t / workers < 1 << 24 || workers > 100) check_totals(t, workers);
+            check_totals(t, workers);
     std::puts("ok");
 }
