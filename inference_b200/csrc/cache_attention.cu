@@ -139,7 +139,8 @@ struct Maps {
 
 template <int NT>
 __global__ void __maxnreg__(NT == 1 ? 128 : 168)
-    cache_attention_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ Maps maps, const Parts parts) {
+    cache_attention_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ Maps maps,
+                           const __grid_constant__ Parts parts) {
     using C = Cfg<NT>;
     constexpr int S = C::kStages;
     extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -464,31 +465,36 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
     }
 }
 
-// The second kernel: joins the parts of cut runs and turns scores into weights.  Its
-// warps take equal contiguous shares of the tiles, each on its own: a warp finds the
-// maximum and sum of every run it meets from that run's parts, writes the weights of
-// its slots, and joins an equal slice of the run's outputs (as many slices as warps
-// that meet the run).  Small enough to be resident beside two CTAs of the first
-// kernel: what depends on the lengths alone happens while that one runs.
+// The second kernel: joins the parts of cut runs and turns scores into weights.  Each
+// CTA takes an equal contiguous share of the tiles: for every run that it meets it finds
+// the maximum and sum from the run's parts, joins a slice of the run's outputs (as many
+// slices as CTAs that meet the run) and writes the weights of its own slots.  Two CTAs an
+// SM, small enough to be resident beside two of the first kernel: what depends on the
+// lengths alone (the share's runs) is done while that one runs.
 constexpr int kJoinThreads = 128;
 constexpr int kJoinWarps = kJoinThreads / 32;
-constexpr int kJoinCtas = 8;  // an SM
+constexpr int kJoinTiles = 64;  // tiles whose runs are looked up at a time, a thread each
+constexpr int kJoinRuns = 8;    // runs joined between two barriers
 struct JoinSmem {
-    float2 ml[kJoinWarps][16];  // of the run at hand: maximum, 1 / sum (0: a bad page, no weights)
+    int4 where[kJoinTiles];                      // of a run met: row, head, first tile here, slots here
+    int4 span[kJoinTiles];                       // its first tile of all, its tiles, first and last chunk's place
+    float2 part[kJoinRuns][kJoinWarps][16];      // each warp's maximum and sum
+    float2 ml[kJoinRuns][16];                    // maximum, 1 / sum (0: a bad page, no weights)
     int before[kJoinThreads + 1];
     int scan[kJoinWarps];
+    unsigned starts[kJoinTiles / 32];
 };
 
 // Weights of n slots from their scores: w[j] += sum_h 2^(s[j][h] - m_h) / l_h.  GV: the
-// heads (0: any number, in `heads`); U slots a lane in flight.
+// heads (0: any number, in `heads`); U slots a thread in flight.
 template <int GV, int U>
-__device__ __forceinline__ void add_weights(float* w, const float* s, const float2* ml, int n, int heads, int lane) {
+__device__ __forceinline__ void add_weights(float* w, const float* s, const float2* ml, int n, int heads) {
     const int G = GV ? GV : heads;
-    for (int j0 = 0; j0 < n; j0 += 32 * U) {
+    for (int j0 = 0; j0 < n; j0 += kJoinThreads * U) {
         float x[U], sc[U][GV ? GV : 1];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * 32 + lane;
+            const int j = j0 + u * kJoinThreads + static_cast<int>(threadIdx.x);
             x[u] = j < n ? w[j] : 0.f;
             if constexpr (GV > 0) {
 #pragma unroll
@@ -509,7 +515,7 @@ __device__ __forceinline__ void add_weights(float* w, const float* s, const floa
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * 32 + lane;
+            const int j = j0 + u * kJoinThreads + static_cast<int>(threadIdx.x);
             float p = 0.f;
             if constexpr (GV > 0) {
 #pragma unroll
@@ -522,129 +528,173 @@ __device__ __forceinline__ void add_weights(float* w, const float* s, const floa
     }
 }
 
+// Maximum and sum of two parts, in this order.  An infinite maximum with the sum 0 marks
+// a bad page (no scores give it: the sum to an infinite maximum is NaN) and spreads.
+__device__ __forceinline__ bool bad_page(float2 v) { return v.x == INFINITY && v.y == 0.f; }
+__device__ __forceinline__ float2 join_ml(float2 x, float2 y) {
+    if (bad_page(x)) return x;
+    if (bad_page(y)) return y;
+    const float m = fmaxf(x.x, y.x), base = m == -INFINITY ? 0.f : m;
+    return make_float2(m, x.y * exp2f(x.x - base) + y.y * exp2f(y.x - base));
+}
+
 __global__ void __maxnreg__(64)
-    cache_join_kernel(const __grid_constant__ CacheAttnArgs a, const Parts parts) {
+    cache_join_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ Parts parts) {
     __shared__ JoinSmem sm;
     const CacheView& c = a.c;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, me = blockIdx.x;
     const int G = a.q_heads / c.kv_heads;
     scan_rows<kJoinThreads>(a.lens, c, sm.before, sm.scan);
     const int total = sm.before[kJoinThreads] * c.kv_heads;
     const Plan plan = plan_make(total, parts.workers);
-    // neighbouring shares on different SMs
-    const int shares = gridDim.x * kJoinWarps, me = warp * gridDim.x + blockIdx.x;
-    const Equal mine = equal_make(total, shares);
-    int t = equal_first(mine, me);
-    const int t1 = equal_first(mine, me + 1);
-    PlanPlace p;
-    int c0 = 0, c1 = 0;
-    auto enter_run = [&]() {  // the run of tile t
-        p = locate<kJoinThreads>(t, a.lens, c, sm.before);
-        c0 = plan_place_of(plan, t - p.tile);
-        c1 = plan_place_of(plan, t - p.tile + p.tiles - 1);
-    };
-    if (t < t1) enter_run();
-    pdl_wait();
-    if (me == 0 && lane == 0) *c.next_chunk = 0;  // for the cache's next attention
-    float2* ml = sm.ml[warp];
-    while (t < t1) {
-        const int run0 = t - p.tile, end = min(t1, run0 + p.tiles);
-        // the run begins in chunk c0: its part there is in slot 1, the others' in slot 0
-        auto part_of = [&](int chunk) { return static_cast<size_t>(chunk * 2 + (chunk == c0 ? 1 : 0)) * G; };
-        const bool cut = c0 != c1;
-        __syncwarp();
-        if (!cut) {
-            if (a.accumulate && lane < G) ml[lane] = parts.ml[static_cast<size_t>(p.row) * a.q_heads + p.head * G + lane];
-        } else {
-            // lane: head lane % wide of every (32 / wide)-th part, wide the power of two that holds G
-            const int wide = G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : G <= 8 ? 8 : 16;
-            const int h = lane % wide, deal = 32 / wide;
-            float M = -INFINITY, L = 0.f;
-            bool bad = false;
-            if (h < G)
-                for (int s0 = c0 + lane / wide; s0 <= c1; s0 += 4 * deal) {
-                    float2 v[4];
-#pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        v[u] = s0 + u * deal <= c1 ? parts.pml[part_of(s0 + u * deal) + h] : make_float2(-INFINITY, 0.f);
-                    float m = M;
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        bad = bad || (v[u].x == INFINITY && v[u].y == 0.f);
-                        m = fmaxf(m, v[u].x);
-                    }
-                    const float base = m == -INFINITY ? 0.f : m;
-                    L *= exp2f(M - base);
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) L += v[u].y * exp2f(v[u].x - base);
-                    M = m;
-                }
-            for (int off = wide; off < 32; off <<= 1) {
-                const float m2 = __shfl_xor_sync(0xffffffffu, M, off), l2 = __shfl_xor_sync(0xffffffffu, L, off);
-                const float m = fmaxf(M, m2), base = m == -INFINITY ? 0.f : m;
-                // the same order of the two on both sides
-                const float x = L * exp2f(M - base), y = l2 * exp2f(m2 - base);
-                L = (lane & off) ? y + x : x + y;
-                M = m;
+    const Equal mine = equal_make(total, gridDim.x);
+    const int t0 = equal_first(mine, me), t1 = equal_first(mine, me + 1);
+    // the runs met by tiles [t, t + 64) of the share
+    int runs = 0;
+    auto look_up = [&](int t) {
+        const int n = min(kJoinTiles, t1 - t);
+        PlanPlace p;
+        bool starts = false;
+        if (tid < kJoinTiles) {
+            if (tid < n) {
+                p = locate<kJoinThreads>(t + tid, a.lens, c, sm.before);
+                starts = tid == 0 || p.tile == 0;
             }
-            bad = __any_sync(0xffffffffu, bad);
-            if (lane < G) ml[lane] = make_float2(M == -INFINITY ? 0.f : M, bad ? 0.f : 1.f / L);
+            const unsigned who = __ballot_sync(0xffffffffu, starts);
+            if (lane == 0) sm.starts[warp] = who;
         }
-        __syncwarp();
-        if (cut) {
-            // outputs in units of 4 dims, lanes: unit lane % wide of every (32 / wide)-th part
-            const int first = equal_share_of(mine, run0), units = G * kCacheHd / 4;
-            const Equal slice = equal_make(units, equal_share_of(mine, run0 + p.tiles - 1) - first + 1);
-            const int u0 = equal_first(slice, me - first), u1 = equal_first(slice, me - first + 1);
-            int wide = 1;
-            while (wide < u1 - u0 && wide < 32) wide *= 2;
-            const int deal = 32 / wide;
-            for (int u = u0; u < u1; u += wide) {
-                const int unit = u + lane % wide;
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                const int h = min(unit, u1 - 1) / (kCacheHd / 4);
-                const float base = ml[h].x, inv = ml[h].y;
-                if (unit < u1)
-#pragma unroll 4
-                    for (int s = c0 + lane / wide; s <= c1; s += deal) {
-                        const size_t at = part_of(s) + h;
-                        const float f = exp2f(parts.pml[at].x - base);
-                        const float4 v = reinterpret_cast<const float4*>(parts.po + at * kCacheHd)[unit % (kCacheHd / 4)];
-                        x.x += v.x * f, x.y += v.y * f, x.z += v.z * f, x.w += v.w * f;
+        __syncthreads();
+        runs = __popc(sm.starts[0]) + __popc(sm.starts[1]);
+        if (starts) {
+            const int at = __popc(sm.starts[warp] & ((1u << lane) - 1)) + (warp ? __popc(sm.starts[0]) : 0);
+            const int run0 = t + tid - p.tile, here = min(n - tid, p.tiles - p.tile);
+            sm.where[at] = make_int4(p.row, p.head, p.tile, min(here * kCachePage, p.len - p.tile * kCachePage));
+            sm.span[at] = make_int4(run0, p.tiles, plan_place_of(plan, run0), plan_place_of(plan, run0 + p.tiles - 1));
+        }
+        __syncthreads();
+    };
+    if (t0 < t1) look_up(t0);
+    pdl_wait();
+    if (me == 0 && tid == 0) *c.next_chunk = 0;  // for the cache's next attention
+
+    // heads side by side in a warp: the power of two that holds G
+    const int wide = G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : G <= 8 ? 8 : 16;
+    for (int t = t0; t < t1; t += kJoinTiles) {
+        if (t > t0) look_up(t);
+        for (int r0 = 0; r0 < runs; r0 += kJoinRuns) {
+            const int nr = min(kJoinRuns, runs - r0);
+            // ---- maximum and sum; thread: head tid % wide of every (threads / wide)-th part
+            for (int r = 0; r < nr; ++r) {
+                const int c0 = sm.span[r0 + r].z, c1 = sm.span[r0 + r].w;
+                if (c0 == c1) continue;
+                const int h = tid % wide, deal = kJoinThreads / wide;
+                float2 v = make_float2(-INFINITY, 0.f);
+                if (h < G)
+                    for (int s0 = c0 + tid / wide; s0 <= c1; s0 += 8 * deal) {
+                        float2 x[8];
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const int s = s0 + u * deal;
+                            // the run begins in chunk c0: its part there is in slot 1, the others' in slot 0
+                            x[u] = s <= c1 ? parts.pml[static_cast<size_t>(s * 2 + (s == c0)) * G + h]
+                                           : make_float2(-INFINITY, 0.f);
+                        }
+                        float m = v.x;
+                        bool bad = bad_page(v);
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            bad = bad || bad_page(x[u]);
+                            m = fmaxf(m, x[u].x);
+                        }
+                        const float base = m == -INFINITY ? 0.f : m;
+                        float l = v.y * exp2f(v.x - base);
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) l += x[u].y * exp2f(x[u].x - base);
+                        v = bad ? make_float2(INFINITY, 0.f) : make_float2(m, l);
                     }
                 for (int off = wide; off < 32; off <<= 1) {
-                    x.x += __shfl_xor_sync(0xffffffffu, x.x, off);
-                    x.y += __shfl_xor_sync(0xffffffffu, x.y, off);
-                    x.z += __shfl_xor_sync(0xffffffffu, x.z, off);
-                    x.w += __shfl_xor_sync(0xffffffffu, x.w, off);
+                    const float2 w =
+                        make_float2(__shfl_xor_sync(0xffffffffu, v.x, off), __shfl_xor_sync(0xffffffffu, v.y, off));
+                    v = (lane & off) ? join_ml(w, v) : join_ml(v, w);  // the same order on both sides
                 }
-                if (lane < wide && unit < u1) {
-                    if (inv == 0.f) x = make_float4(NAN, NAN, NAN, NAN);
-                    const float k = inv == 0.f ? 1.f : inv;
-                    uint2 o;
-                    o.x = pack_bf2(f2bf(x.x * k), f2bf(x.y * k));
-                    o.y = pack_bf2(f2bf(x.z * k), f2bf(x.w * k));
-                    reinterpret_cast<uint2*>(a.out + p.row * a.out_stride + static_cast<size_t>(p.head) * G * kCacheHd)[unit] = o;
+                if (lane < wide) sm.part[r][warp][lane] = v;
+            }
+            __syncthreads();
+            {
+                const int r = tid >> 4, h = tid & 15;
+                if (r < nr && h < G) {
+                    const int4 w = sm.where[r0 + r], sp = sm.span[r0 + r];
+                    if (sp.z == sp.w) {
+                        if (a.accumulate)
+                            sm.ml[r][h] = parts.ml[static_cast<size_t>(w.x) * a.q_heads + w.y * G + h];
+                    } else {
+                        float2 v = sm.part[r][0][h];
+#pragma unroll
+                        for (int i = 1; i < kJoinWarps; ++i) v = join_ml(v, sm.part[r][i][h]);
+                        sm.ml[r][h] = make_float2(v.x == -INFINITY ? 0.f : v.x, bad_page(v) ? 0.f : 1.f / v.y);
+                    }
                 }
             }
-        }
-        if (a.accumulate) {
-            bool bad = false;
-            for (int h = 0; h < G; ++h) bad = bad || ml[h].y == 0.f;
-            const int n = min((end - t) * kCachePage, p.len - p.tile * kCachePage);
-            float* w = c.weights + cache_slot_index(c, p.row, p.head) + p.tile * kCachePage;
-            const float* s = parts.score + static_cast<size_t>(t) * kCachePage * G;
-            if (!bad) switch (G) {
-                    case 1: add_weights<1, 8>(w, s, ml, n, G, lane); break;
-                    case 2: add_weights<2, 8>(w, s, ml, n, G, lane); break;
-                    case 4: add_weights<4, 4>(w, s, ml, n, G, lane); break;
-                    case 8: add_weights<8, 4>(w, s, ml, n, G, lane); break;
-                    case 16: add_weights<16, 2>(w, s, ml, n, G, lane); break;
-                    default: add_weights<0, 2>(w, s, ml, n, G, lane);
+            __syncthreads();
+            // ---- outputs of cut runs, in units of 4 dims: a warp takes units, its lanes their parts
+            for (int r = 0; r < nr; ++r) {
+                const int4 w = sm.where[r0 + r], sp = sm.span[r0 + r];
+                if (sp.z == sp.w || max(sp.x, t0) != sp.x + w.z) continue;  // whole, or met before in this share
+                const int first = equal_share_of(mine, sp.x), units = G * kCacheHd / 4;
+                const Equal slice = equal_make(units, equal_share_of(mine, sp.x + sp.y - 1) - first + 1);
+                const int u0 = equal_first(slice, me - first), u1 = equal_first(slice, me - first + 1);
+                const int P = sp.w - sp.z + 1;
+                const int turns = P <= 2 ? 2 : P <= 4 ? 4 : P <= 8 ? 8 : P <= 16 ? 16 : 32;
+                const int width = 32 / turns, turn = lane / width;
+                for (int u = u0 + warp * width; u < u1; u += kJoinWarps * width) {
+                    const int unit = u + lane % width, h = min(unit, u1 - 1) / (kCacheHd / 4);
+                    const float2 ml = sm.ml[r][h];
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (unit < u1)
+#pragma unroll 4
+                        for (int s = sp.z + turn; s <= sp.w; s += turns) {
+                            const size_t at = static_cast<size_t>(s * 2 + (s == sp.z)) * G + h;
+                            const float f = exp2f(parts.pml[at].x - ml.x);
+                            const float4 v = reinterpret_cast<const float4*>(parts.po + at * kCacheHd)[unit % (kCacheHd / 4)];
+                            x.x += v.x * f, x.y += v.y * f, x.z += v.z * f, x.w += v.w * f;
+                        }
+                    for (int off = width; off < 32; off <<= 1) {
+                        x.x += __shfl_xor_sync(0xffffffffu, x.x, off);
+                        x.y += __shfl_xor_sync(0xffffffffu, x.y, off);
+                        x.z += __shfl_xor_sync(0xffffffffu, x.z, off);
+                        x.w += __shfl_xor_sync(0xffffffffu, x.w, off);
+                    }
+                    if (turn == 0 && unit < u1) {
+                        if (ml.y == 0.f) x = make_float4(NAN, NAN, NAN, NAN);
+                        const float k = ml.y == 0.f ? 1.f : ml.y;
+                        uint2 o;
+                        o.x = pack_bf2(f2bf(x.x * k), f2bf(x.y * k));
+                        o.y = pack_bf2(f2bf(x.z * k), f2bf(x.w * k));
+                        reinterpret_cast<uint2*>(a.out + w.x * a.out_stride + static_cast<size_t>(w.y) * G * kCacheHd)[unit] = o;
+                    }
                 }
+            }
+            // ---- weights
+            if (a.accumulate)
+                for (int r = 0; r < nr; ++r) {
+                    const int4 w = sm.where[r0 + r];
+                    const float2* ml = sm.ml[r];
+                    bool bad = false;
+                    for (int h = 0; h < G; ++h) bad = bad || ml[h].y == 0.f;
+                    if (bad) continue;
+                    float* to = c.weights + cache_slot_index(c, w.x, w.y) + w.z * kCachePage;
+                    const float* s = parts.score + static_cast<size_t>(sm.span[r0 + r].x + w.z) * kCachePage * G;
+                    switch (G) {
+                        case 1: add_weights<1, 8>(to, s, ml, w.w, G); break;
+                        case 2: add_weights<2, 6>(to, s, ml, w.w, G); break;
+                        case 4: add_weights<4, 4>(to, s, ml, w.w, G); break;
+                        case 8: add_weights<8, 2>(to, s, ml, w.w, G); break;
+                        case 16: add_weights<16, 1>(to, s, ml, w.w, G); break;
+                        default: add_weights<0, 2>(to, s, ml, w.w, G);
+                    }
+                }
+            __syncthreads();  // sm.ml and sm.part are the next runs'
         }
-        t = end;
-        if (t < t1) enter_run();
     }
 }
 
@@ -730,7 +780,7 @@ cudaError_t launch_cache_attention(const CacheAttnArgs& a, int sms, cudaStream_t
     cudaError_t e = a.q_heads / c.kv_heads <= 8 ? launch_nt<1>(a, maps, parts, s) : launch_nt<2>(a, maps, parts, s);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min(static_cast<size_t>(kJoinCtas * sms), (max_tiles(c) + kJoinWarps - 1) / kJoinWarps)));
+    cfg.gridDim = dim3(parts.workers);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];

@@ -23,6 +23,21 @@ namespace q3 {
 constexpr int kPlanTile = 64;
 constexpr int kPlanSmall = 3;  // no chunk but a region's last is smaller than this many tiles
 
+// n / d for 0 <= n < 2^31, d > 0: on the device by way of a float quotient and its
+// correction, a third of the latency of the general division.
+Q3_HD int plan_div(int n, int d) {
+#ifdef __CUDA_ARCH__
+    int q = static_cast<int>(static_cast<float>(n) * __frcp_rn(static_cast<float>(d)));
+    // the float quotient may be off by a little either way, and n = q * d must not wrap
+    long long r = static_cast<long long>(n) - static_cast<long long>(q) * d;
+    while (r < 0) --q, r += d;
+    while (r >= d) ++q, r -= d;
+    return q;
+#else
+    return n / d;
+#endif
+}
+
 Q3_HD int plan_tiles(int len, int max_len) {
     return len > 0 && len <= max_len ? (len + kPlanTile - 1) / kPlanTile : 0;
 }
@@ -34,14 +49,14 @@ struct Equal {
 };
 Q3_HD Equal equal_make(int total, int parts) {
     Equal e;
-    e.base = total / parts;
+    e.base = plan_div(total, parts);
     e.extra = total - e.base * parts;
     return e;
 }
 Q3_HD int equal_first(const Equal& e, int i) { return i * e.base + (i < e.extra ? i : e.extra); }
 Q3_HD int equal_share_of(const Equal& e, int t) {
     const int big = e.extra * (e.base + 1);
-    return t < big ? t / (e.base + 1) : e.extra + (t - big) / e.base;
+    return t < big ? plan_div(t, e.base + 1) : e.extra + plan_div(t - big, e.base);
 }
 
 // Every worker (CTA) has an equal region of the tiles.  Its first 5/8 are one chunk,
@@ -98,8 +113,8 @@ struct PlanPlace {
 };
 Q3_HD PlanPlace plan_locate(int t, const int32_t* lens, int rows, int max_len, int kv_heads, const int* before,
                             int groups) {
-    const int u = t / kv_heads;  // lies in the row that holds tile u of one head
-    int lo = 0, hi = groups;     // before[lo] <= u < before[hi]
+    const int u = plan_div(t, kv_heads);  // lies in the row that holds tile u of one head
+    int lo = 0, hi = groups;              // before[lo] <= u < before[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (before[mid] <= u)
@@ -118,7 +133,7 @@ Q3_HD PlanPlace plan_locate(int t, const int32_t* lens, int rows, int max_len, i
         ++p.row;
     }
     const int rem = t - first * kv_heads;
-    p.head = rem / p.tiles;
+    p.head = plan_div(rem, p.tiles);
     p.tile = rem - p.head * p.tiles;
     return p;
 }
