@@ -181,6 +181,7 @@ int q3_cache_create(const q3_cache_desc* d, int device, q3_cache** out) {
     v.kv_heads = static_cast<int>(d->kv_heads);
     v.err = d->state_dev;
     v.next_chunk = d->state_dev + 1;
+    v.arrived = d->state_dev + 2;
     *out = c;
     return Q3_OK;
 }
@@ -199,7 +200,8 @@ int q3_cache_sync(q3_cache* c, void* stream) {
     Q3_CUDA(cudaMemcpyAsync(&code, c->view.err, 4, cudaMemcpyDeviceToHost, s));
     Q3_CUDA(cudaStreamSynchronize(s));
     if (code == DEV_OK) return Q3_OK;
-    Q3_CUDA(cudaMemsetAsync(c->view.err, 0, 4, s));
+    // the work counters with it: a kernel that gave up may have left them anywhere
+    Q3_CUDA(cudaMemsetAsync(c->view.err, 0, Q3_CACHE_STATE_WORDS * 4, s));
     Q3_CUDA(cudaStreamSynchronize(s));
     return fail(Q3_ERR_DEVICE, std::string("q3_cache: ") + device_error_text(code));
 }
@@ -327,7 +329,7 @@ int q3_cache_evict(q3_cache* c, const int32_t* lens, const int32_t* next_pos, si
     a.positions_out = positions_out;
     a.lens_out = lens_out;
     a.ws = ws;
-    return launched(launch_cache_evict(a, static_cast<cudaStream_t>(stream)), "q3_cache_evict");
+    return launched(launch_cache_evict(a, c->sms, static_cast<cudaStream_t>(stream)), "q3_cache_evict");
 }
 
 }  // extern "C"

@@ -21,7 +21,8 @@ struct CacheView {
     int32_t* positions;
     long long slot_stride;
     int rows, max_len, kv_heads;
-    uint32_t *err, *next_chunk;  // q3_cache_desc.state_dev: the error word; chunks taken by the attention running
+    // q3_cache_desc.state_dev: the error word; the attention's chunks taken; the eviction's CTAs arrived
+    uint32_t *err, *next_chunk, *arrived;
 };
 
 __host__ __device__ inline size_t cache_slot_index(const CacheView& c, int row, int head) {
@@ -70,6 +71,6 @@ struct CacheEvictArgs {
     void* ws;
 };
 size_t cache_evict_ws_bytes(const CacheView& c, int keep);
-cudaError_t launch_cache_evict(const CacheEvictArgs& a, cudaStream_t s);
+cudaError_t launch_cache_evict(const CacheEvictArgs& a, int sms, cudaStream_t s);
 
 }  // namespace q3
