@@ -9,16 +9,17 @@
 // in front.
 //
 // One thread-block cluster per (sequence, kv head), each CTA a contiguous piece of
-// its slots.  The `keep`-th largest key is found by a radix
-// select over 52 bits, weight above (inverted) slot, so that no two keys are
-// equal: 2048-bin histograms of 11 bits a pass, summed over the cluster through
-// distributed shared memory, until at most 256 candidates are left, which are
-// ranked by counting (one or two passes for weights of a usual spread).  Then a
-// bitmap of the kept slots, the ordered lists of holes and movers from its
-// population counts, and the moves, 16 lanes a slot and tensor: by the same CTAs
-// where at most 64 slots a head can move, else by a second launch over all SMs.
-// Bound: latency (a dozen dependent steps of 0.3 to 0.5 us) for a few evicted
-// slots, HBM for many: 8 bytes a slot read, 1 KB a moved slot.
+// its slots.  The weight of the `keep`-th slot is found by a radix select over the
+// weights' 32-bit order-preserving keys: a histogram of the next 11 bits (8 in a
+// cluster, whose CTAs read each other's through distributed shared memory) of the
+// slots that share the bits so far, until at most 256 candidates are left, which are
+// ranked by counting; usually one or two passes.  More candidates than that with all
+// bits equal are a tie, cut by slot.  Then a bitmap of the kept slots, the ordered
+// lists of holes and movers from its population counts, and the moves, 16 lanes a
+// slot and tensor: by the same CTAs where at most 64 slots a head can move, else by
+// a second launch over all SMs.  Bound: latency (a dozen dependent steps of 0.3 to
+// 0.7 us) for a few evicted slots, HBM for many: 8 bytes a slot read, 1 KB a moved
+// slot.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -31,28 +32,19 @@ namespace {
 constexpr int kThreads = 512;               // two CTAs an SM
 constexpr int kWarps = kThreads / 32;
 constexpr int kHeld = 8;                    // slots a thread holds in registers (more are read again in every pass)
-constexpr int kDigit = 11;                  // bits a pass
-constexpr int kBins = 1 << kDigit;
-constexpr int kSlotBits = 20;               // max_len <= 2^20
-constexpr int kTopShift = 32 + kSlotBits - kDigit;
 constexpr int kCandidates = 256;
 constexpr int kMaxCluster = 8;
 constexpr int kMovesHere = 64;  // at most so many moves a head: by the selecting CTAs
 constexpr int kMoveThreads = 256;
 constexpr int kMoveChunk = 64;
-static_assert(kBins == 4 * kThreads && kCandidates * 2 == kThreads, "bins and candidates are dealt to the threads");
+static_assert(kCandidates * 2 == kThreads, "two threads rank a candidate");
 
 // Larger key = kept earlier.  Slots of the recent window come before every
-// number, NaN after every number, and -0 equals +0; among equals the lower slot.
-__device__ __forceinline__ uint64_t evict_key(float w, bool recent, int slot) {
-    uint32_t k = 0u;
-    if (recent) {
-        k = 0xFFFFFFFFu;
-    } else if (!isnan(w)) {
-        const uint32_t b = __float_as_uint(w + 0.0f);
-        k = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-    }
-    return (static_cast<uint64_t>(k) << kSlotBits) | static_cast<uint32_t>((1 << kSlotBits) - 1 - slot);
+// number, NaN after every number, and -0 equals +0.
+__device__ __forceinline__ uint32_t evict_key(float w, bool recent) {
+    const uint32_t b = __float_as_uint(w + 0.0f);
+    const uint32_t k = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+    return recent ? 0xFFFFFFFFu : isnan(w) ? 0u : k;
 }
 
 // A slot and the row of the K and V pools that holds it: (page * kv_heads + head) * 64 + slot % 64.
@@ -63,17 +55,27 @@ struct Lists {
     int cap;
 };
 
+// Histogram digits: 11 bits for one CTA; 8 in a cluster, where every CTA reads every
+// peer's histogram (at 11 bits that alone took 2 us a pass with 8 CTAs).
+template <int C>
+struct Digits {
+    static constexpr int kBits = C == 1 ? 11 : 8;
+    static constexpr int kBins = 1 << kBits;
+    static constexpr int kPer = C == 1 ? 4 : 1;  // bins a thread
+};
+
 struct Smem {
-    int hist[2][kBins];  // alternately: one is cleared while peers may still read the other
+    int hist[2][2048];  // alternately: one is cleared while peers may still read the other
     uint64_t mine[kCandidates], all[kCandidates];
     int2 dst[kMovesHere], src[kMovesHere];
     int n_mine;
     int warp_sum[kWarps];
     int warp_holes[kWarps], warp_movers[kWarps];
-    int holes, movers;       // of this CTA's piece
-    int digit, need, count;  // the bin that holds the threshold
-    uint64_t threshold;
-    uint32_t kept[];  // bitmap of the piece
+    int holes, movers, ties;  // of this CTA's piece
+    int digit, need, count;   // the bin that holds the threshold
+    uint32_t key;             // kept: a larger key, or this key and a slot up to
+    int slot;                 // this one
+    uint32_t kept[];          // bitmap of the piece
 };
 
 // Moves i = first, first + step, ... below n, each by the 16 lanes that share `first`:
@@ -140,42 +142,45 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     const float* w = c.weights + at;
     const int32_t* pos = c.positions + at;
     if (!moves_here) pdl_trigger();
-    for (int i = tid; i < kBins; i += kThreads) sm.hist[0][i] = 0;
+    using D = Digits<C>;
+    for (int i = tid; i < D::kBins; i += kThreads) sm.hist[0][i] = 0;
     if (tid == 0) sm.n_mine = 0;
 
     // the piece: words of 32 slots, a warp a contiguous run of them
     const bool length_ok = len >= 0 && len <= c.max_len, shrinks = length_ok && len > a.keep;
     const int words = length_ok ? (len + 31) / 32 : 0;
-    const int word0 = static_cast<int>(static_cast<long long>(words) * rank / C);
-    const int nw = static_cast<int>(static_cast<long long>(words) * (rank + 1) / C) - word0;
+    const int word0 = words / C * rank + words % C * rank / C;
+    const int nw = words / C * (rank + 1) + words % C * (rank + 1) / C - word0;
     const int wa = nw * warp / kWarps, wb = nw * (warp + 1) / kWarps;
-    float hx[kHeld];
-    int32_t hp[kHeld];
+    // lane's slot of word i of the piece, and its key (0 for a slot behind the length: never the only
+    // reason to keep it, since such slots are masked out)
+    auto slot_of = [&](int i) { return (word0 + i) * 32 + lane; };
+    auto key_of = [&](int s) { return s < len ? evict_key(w[s], pos[s] >= first_recent) : 0u; };
+    uint32_t held[kHeld];
+    if (shrinks) {
+        float x[kHeld];
+        int32_t p[kHeld];
 #pragma unroll
-    for (int u = 0; u < kHeld; ++u) {
-        const int s = (word0 + wa + u) * 32 + lane;
-        const bool in = wa + u < wb && s < len;
-        hx[u] = in ? w[s] : 0.f;
-        hp[u] = in ? pos[s] : 0;
+        for (int u = 0; u < kHeld; ++u) {
+            const bool in = wa + u < wb && slot_of(wa + u) < len;
+            x[u] = in ? w[slot_of(wa + u)] : 0.f;
+            p[u] = in ? pos[slot_of(wa + u)] : INT_MIN;
+        }
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) held[u] = evict_key(x[u], p[u] >= first_recent);
     }
-    // f(word of the piece, slot, weight, position) for the warp's words, by the whole warp
+    // f(word of the piece, slot, key) for the warp's words, by the whole warp
     auto each_word = [&](auto&& f) {
 #pragma unroll
         for (int u = 0; u < kHeld; ++u)
-            if (wa + u < wb) f(wa + u, (word0 + wa + u) * 32 + lane, hx[u], hp[u]);
+            if (wa + u < wb) f(wa + u, slot_of(wa + u), held[u]);
         for (int i = wa + kHeld; i < wb; i += 4) {
-            float x[4];
-            int32_t p[4];
+            uint32_t k[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int s = (word0 + i + u) * 32 + lane;
-                const bool in = i + u < wb && s < len;
-                x[u] = in ? w[s] : 0.f;
-                p[u] = in ? pos[s] : 0;
-            }
+            for (int u = 0; u < 4; ++u) k[u] = i + u < wb ? key_of(slot_of(i + u)) : 0u;
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (i + u < wb) f(i + u, (word0 + i + u) * 32 + lane, x[u], p[u]);
+                if (i + u < wb) f(i + u, slot_of(i + u), k[u]);
         }
     };
     uint32_t bad = length_ok ? DEV_OK : DEV_BAD_LENGTH;
@@ -207,48 +212,43 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     if (stays || !shrinks) {
         if (tid == 0 && rank == 0) m.count[rh] = 0;
         if (!stays && a.weights_out)
-            each_word([&](int, int s, float x, int32_t p) {
-                if (s < len) a.weights_out[at + s] = x, a.positions_out[at + s] = p;
-            });
+            for (int s = word0 * 32 + tid; s < min(len, (word0 + nw) * 32); s += kThreads) {
+                a.weights_out[at + s] = w[s];
+                a.positions_out[at + s] = pos[s];
+            }
         finish();
         return;
     }
 
-    // ---- the threshold: the keep-th largest key
-    uint64_t prefix = 0;
-    int need = a.keep;
-    // at the last shift, 8, at most 256 slots share a prefix: the loop ends by a break
-    for (int pass = 0, shift = kTopShift; shift >= 0; ++pass, shift -= kDigit) {
+    // ---- the threshold: the keep-th largest key, and among equals the last slot kept
+    uint32_t prefix = 0;  // the keys' bits above the shift
+    int need = a.keep, count = len;
+    bool found = false;
+    for (int pass = 0, shift = 32 - D::kBits, bits = D::kBits; !found && bits > 0; ++pass) {
         int* hist = sm.hist[pass & 1];
         if (pass > 0) {
-            for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
+            for (int i = tid; i < D::kBins; i += kThreads) hist[i] = 0;
             __syncthreads();
         }
-        each_word([&](int, int s, float x, int32_t p) {
-            const uint64_t k = evict_key(x, p >= first_recent, s);
-            const bool in = s < len && (k >> (shift + kDigit)) == prefix;
-            const unsigned here = __ballot_sync(0xffffffffu, in);
-            if (!here) return;
-            const int d = static_cast<int>(k >> shift) & (kBins - 1);
-            // lanes with one digit between them (equal weights) count as one
-            const int first = __ffs(here) - 1;
-            const int theirs = __shfl_sync(0xffffffffu, d, first);
-            const bool same = __all_sync(0xffffffffu, !in || d == theirs) != 0;
-            if (!same) {
-                if (in) atomicAdd(&hist[d], 1);
-            } else if (lane == first) {
-                atomicAdd(&hist[d], __popc(here));
-            }
+        each_word([&](int, int s, uint32_t k) {
+            const uint32_t top = k >> shift;
+            if (s < len && (pass == 0 || top >> bits == prefix)) atomicAdd(&hist[top & ((1u << bits) - 1)], 1);
         });
         cluster_sync<C>();
-        // thread t has the bins 2047 - 4 t - i, i = 0 .. 3, from the top
-        int4 part[C];
-#pragma unroll
-        for (int r = 0; r < C; ++r)
-            part[r] = reinterpret_cast<const int4*>(C == 1 ? hist : peer(hist, r))[kBins / 4 - 1 - tid];
+        // thread t has the kPer bins from kBins - 1 - kPer t downwards
         int four[4] = {0, 0, 0, 0};
+        if (tid < D::kBins / D::kPer) {
+            if constexpr (C == 1) {
+                const int4 h = reinterpret_cast<const int4*>(hist)[D::kBins / 4 - 1 - tid];
+                four[0] = h.w, four[1] = h.z, four[2] = h.y, four[3] = h.x;
+            } else {
+                int h[C];
 #pragma unroll
-        for (int r = 0; r < C; ++r) four[0] += part[r].w, four[1] += part[r].z, four[2] += part[r].y, four[3] += part[r].x;
+                for (int r = 0; r < C; ++r) h[r] = peer(hist, r)[D::kBins - 1 - tid];
+#pragma unroll
+                for (int r = 0; r < C; ++r) four[0] += h[r];
+            }
+        }
         const int all = four[0] + four[1] + four[2] + four[3];
         int incl = all;
 #pragma unroll
@@ -261,24 +261,23 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
         // larger than this thread's bins: the warps and lanes before
         int above = __reduce_add_sync(0xffffffffu, lane < warp ? sm.warp_sum[lane & (kWarps - 1)] : 0) + incl - all;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < D::kPer; ++i) {
             if (above < need && need <= above + four[i])
-                sm.digit = kBins - 1 - 4 * tid - i, sm.need = need - above, sm.count = four[i];
+                sm.digit = D::kBins - 1 - D::kPer * tid - i, sm.need = need - above, sm.count = four[i];
             above += four[i];
         }
         __syncthreads();
-        prefix = (prefix << kDigit) | static_cast<uint64_t>(sm.digit);
+        prefix = (prefix << bits) | static_cast<uint32_t>(sm.digit);
         need = sm.need;
-        const int count = sm.count;
+        count = sm.count;
         if (count == need) {  // the whole bin is kept
-            if (tid == 0) sm.threshold = prefix << shift;
-            break;
-        }
-        if (count <= kCandidates) {
-            // few candidates: the one with need - 1 larger ones is the threshold
-            each_word([&](int, int s, float x, int32_t p) {
-                const uint64_t k = evict_key(x, p >= first_recent, s);
-                if (s < len && (k >> shift) == prefix) sm.mine[atomicAdd(&sm.n_mine, 1)] = k;
+            if (tid == 0) sm.key = prefix << shift, sm.slot = INT_MAX;
+            found = true;
+        } else if (count <= kCandidates) {
+            // few candidates: the one with need - 1 larger ones (the lower slot is the larger) is the last kept
+            each_word([&](int, int s, uint32_t k) {
+                if (s < len && k >> shift == prefix)
+                    sm.mine[atomicAdd(&sm.n_mine, 1)] = (static_cast<uint64_t>(k) << 32) | static_cast<uint32_t>(~s);
             });
             cluster_sync<C>();
             const uint64_t* from = sm.mine;
@@ -294,21 +293,58 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
                 from = sm.all;
                 __syncthreads();
             }
-            // two threads a candidate
-            const int i = tid >> 1;
+            const int i = tid >> 1;  // two threads a candidate
             if (i < count) {
                 const uint64_t k = from[i];
                 int larger = 0;
 #pragma unroll 8
                 for (int j = tid & 1; j < count; j += 2) larger += from[j] > k;
                 larger += __shfl_xor_sync(0x3u << (lane & ~1), larger, 1);
-                if (larger == need - 1 && (tid & 1) == 0) sm.threshold = k;
+                if (larger == need - 1 && (tid & 1) == 0)
+                    sm.key = static_cast<uint32_t>(k >> 32), sm.slot = static_cast<int>(~static_cast<uint32_t>(k));
             }
-            break;
+            found = true;
         }
+        // the next digit; none is left when the bin is one key
+        bits = min(D::kBits, shift);
+        shift -= bits;
+    }
+    if (!found) {
+        // more than 256 slots of one key, of which the first `need` are kept: count them by warp
+        int ties = 0;
+        each_word([&](int, int s, uint32_t k) { ties += __popc(__ballot_sync(0xffffffffu, s < len && k == prefix)); });
+        if (lane == 0) sm.warp_sum[warp] = ties;
+        __syncthreads();
+        const int theirs = lane < kWarps ? sm.warp_sum[lane] : 0;
+        int before = __reduce_add_sync(0xffffffffu, lane < warp ? theirs : 0);
+        if constexpr (C > 1) {
+            const int piece = __reduce_add_sync(0xffffffffu, theirs);
+            if (tid == 0) sm.ties = piece;
+            cluster_sync<C>();
+#pragma unroll
+            for (int r = 0; r < C; ++r) {
+                const int n = *peer(&sm.ties, r);
+                if (r < rank) before += n;
+            }
+        }
+        if (before < need && need <= before + ties) {
+            // the need-th is in this warp
+            each_word([&](int, int s, uint32_t k) {
+                const bool tie = s < len && k == prefix;
+                const uint32_t mask = __ballot_sync(0xffffffffu, tie);
+                if (tie && before + __popc(mask & ((2u << lane) - 1)) == need)
+                    for (int r = 0; r < C; ++r) {
+                        Smem* to = C == 1 ? &sm : const_cast<Smem*>(peer(&sm, r));
+                        to->key = prefix, to->slot = s;
+                    }
+                before += __popc(mask);
+            });
+        }
+        if (C > 1) cluster_sync<C>();
     }
     __syncthreads();
-    const uint64_t threshold = sm.threshold;
+    const uint32_t last_key = sm.key;
+    const int last_slot = sm.slot;
 
     // ---- the kept slots' bitmap
     // bit i of the mask: slot 32 * word + i is below keep
@@ -316,19 +352,25 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
         const int n = a.keep - word * 32;
         return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1;
     };
-    int holes = 0, movers = 0;
-    each_word([&](int i, int s, float x, int32_t p) {
-        const bool keep = s < len && evict_key(x, p >= first_recent, s) >= threshold;
-        const uint32_t mask = __ballot_sync(0xffffffffu, keep), low = below(word0 + i);
+    each_word([&](int i, int s, uint32_t k) {
+        const bool keep = s < len && (k > last_key || (k == last_key && s <= last_slot));
+        const uint32_t mask = __ballot_sync(0xffffffffu, keep);
         if (lane == 0) sm.kept[i] = mask;
-        holes += __popc(~mask & low);
-        movers += __popc(mask & ~low);
-        if (a.weights_out && keep && s < a.keep) a.weights_out[at + s] = x, a.positions_out[at + s] = p;
+        if (a.weights_out && keep && s < a.keep) a.weights_out[at + s] = w[s], a.positions_out[at + s] = pos[s];
     });
-    if (lane == 0) sm.warp_holes[warp] = holes, sm.warp_movers[warp] = movers;
+    __syncwarp();
+    int my_holes = 0, my_movers = 0;
+    for (int i = wa + lane; i < wb; i += 32) {
+        const uint32_t mask = sm.kept[i], low = below(word0 + i);
+        my_holes += __popc(~mask & low);
+        my_movers += __popc(mask & ~low);
+    }
+    my_holes = __reduce_add_sync(0xffffffffu, my_holes);
+    my_movers = __reduce_add_sync(0xffffffffu, my_movers);
+    if (lane == 0) sm.warp_holes[warp] = my_holes, sm.warp_movers[warp] = my_movers;
     __syncthreads();
     // lists in order: the pieces before this one, the warps before this one
-    const int my_holes = lane < kWarps ? sm.warp_holes[lane] : 0, my_movers = lane < kWarps ? sm.warp_movers[lane] : 0;
+    my_holes = lane < kWarps ? sm.warp_holes[lane] : 0, my_movers = lane < kWarps ? sm.warp_movers[lane] : 0;
     int hole = __reduce_add_sync(0xffffffffu, lane < warp ? my_holes : 0);
     int mover = __reduce_add_sync(0xffffffffu, lane < warp ? my_movers : 0);
     int n = __reduce_add_sync(0xffffffffu, my_movers);
@@ -352,9 +394,10 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     int2* src = local ? sm.src : m.src + static_cast<size_t>(rh) * m.cap;
     const unsigned lower = (1u << lane) - 1;
     auto place_of = [&](int s) { return make_int2(s, (table[s / kCachePage] * c.kv_heads + head) * kCachePage + s % kCachePage); };
+#pragma unroll 4
     for (int i = wa; i < wb; ++i) {
         const uint32_t mask = sm.kept[i], low = below(word0 + i), h = ~mask & low, v = mask & ~low;
-        const int s = (word0 + i) * 32 + lane;
+        const int s = slot_of(i);
         if (h >> lane & 1) dst[hole + __popc(h & lower)] = place_of(s);
         if (v >> lane & 1) src[mover + __popc(v & lower)] = place_of(s);
         hole += __popc(h);
@@ -403,7 +446,7 @@ cudaError_t launch_select(const CacheEvictArgs& a, const Lists& m, int moves_her
     const uint64_t bit = 1ull << (dev & 63);
     if (!(configured.load() & bit)) {
         e = cudaFuncSetAttribute(cache_evict_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(sizeof(Smem) + ((1 << kSlotBits) / 32 + 2) * 4));
+                                 static_cast<int>(sizeof(Smem) + ((1 << 20) / 32 + 2) * 4));
         if (e != cudaSuccess) return e;
         configured.fetch_or(bit);
     }
