@@ -31,7 +31,8 @@ namespace {
 
 constexpr int kThreads = 512;               // two CTAs an SM
 constexpr int kWarps = kThreads / 32;
-constexpr int kHeld = 8;                    // slots a thread holds in registers (more are read again in every pass)
+constexpr int kKeysHere = 20480;            // a piece's keys stay in shared memory up to so many slots (80 KB: two CTAs an
+                                            // SM), else they are made again in every pass
 constexpr int kCandidates = 256;
 constexpr int kMaxCluster = 8;
 constexpr int kMovesHere = 64;  // at most so many moves a head: by the selecting CTAs
@@ -75,7 +76,7 @@ struct Smem {
     int digit, need, count;   // the bin that holds the threshold
     uint32_t key;             // kept: a larger key, or this key and a slot up to
     int slot;                 // this one
-    uint32_t kept[];          // bitmap of the piece
+    uint32_t words[];         // bitmap of the piece's kept slots, then their keys
 };
 
 // Moves i = first, first + step, ... below n, each by the 16 lanes that share `first`:
@@ -128,7 +129,8 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 template <int C>
-__global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvictArgs a, const Lists m, int moves_here) {
+__global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvictArgs a, const Lists m, int moves_here,
+                                                                  int key_words) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     const CacheView& c = a.c;
@@ -152,41 +154,35 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     const int word0 = words / C * rank + words % C * rank / C;
     const int nw = words / C * (rank + 1) + words % C * (rank + 1) / C - word0;
     const int wa = nw * warp / kWarps, wb = nw * (warp + 1) / kWarps;
-    // lane's slot of word i of the piece, and its key (0 for a slot behind the length: never the only
-    // reason to keep it, since such slots are masked out)
-    auto slot_of = [&](int i) { return (word0 + i) * 32 + lane; };
-    auto key_of = [&](int s) { return s < len ? evict_key(w[s], pos[s] >= first_recent) : 0u; };
-    uint32_t held[kHeld];
-    if (shrinks) {
-        float x[kHeld];
-        int32_t p[kHeld];
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u) {
-            const bool in = wa + u < wb && slot_of(wa + u) < len;
-            x[u] = in ? w[slot_of(wa + u)] : 0.f;
-            p[u] = in ? pos[slot_of(wa + u)] : INT_MIN;
-        }
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u) held[u] = evict_key(x[u], p[u] >= first_recent);
-    }
+    uint32_t* kept = sm.words;
+    uint32_t* keys = key_words ? sm.words + key_words : nullptr;
+    auto slot_of = [&](int i) { return (word0 + i) * 32 + lane; };  // lane's slot of word i of the piece
     // f(word of the piece, slot, key) for the warp's words, by the whole warp
     auto each_word = [&](auto&& f) {
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-            if (wa + u < wb) f(wa + u, slot_of(wa + u), held[u]);
-        for (int i = wa + kHeld; i < wb; i += 4) {
-            uint32_t k[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) k[u] = i + u < wb ? key_of(slot_of(i + u)) : 0u;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (i + u < wb) f(i + u, slot_of(i + u), k[u]);
+#pragma unroll 4
+        for (int i = wa; i < wb; ++i) {
+            const int s = slot_of(i);
+            f(i, s, keys ? keys[i * 32 + lane] : s < len ? evict_key(w[s], pos[s] >= first_recent) : 0u);
         }
     };
+    // four words' weights and positions, ahead of the page check
+    constexpr int U = 4;
+    float x[U];
+    int32_t p[U];
+    auto load_words = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = slot_of(i + u);
+            const bool in = i + u < wb && s < len;
+            x[u] = in ? w[s] : 0.f;
+            p[u] = in ? pos[s] : 0;
+        }
+    };
+    load_words(wa);
     uint32_t bad = length_ok ? DEV_OK : DEV_BAD_LENGTH;
     if (shrinks)
-        for (int p = tid; p < (len + kCachePage - 1) / kCachePage; p += kThreads)
-            if (table[p] < 0 || table[p] >= c.num_pages) bad = DEV_BAD_PAGE;
+        for (int i = tid; i < (len + kCachePage - 1) / kCachePage; i += kThreads)
+            if (table[i] < 0 || table[i] >= c.num_pages) bad = DEV_BAD_PAGE;
     const bool stays = __syncthreads_or(bad) != 0;
     if (bad && rank == 0) record_error(c.err, bad);
 
@@ -212,9 +208,14 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     if (stays || !shrinks) {
         if (tid == 0 && rank == 0) m.count[rh] = 0;
         if (!stays && a.weights_out)
-            for (int s = word0 * 32 + tid; s < min(len, (word0 + nw) * 32); s += kThreads) {
-                a.weights_out[at + s] = w[s];
-                a.positions_out[at + s] = pos[s];
+            for (int i = wa; i < wb; i += U) {
+                if (i > wa) load_words(i);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (i + u < wb && slot_of(i + u) < len) {
+                        a.weights_out[at + slot_of(i + u)] = x[u];
+                        a.positions_out[at + slot_of(i + u)] = p[u];
+                    }
             }
         finish();
         return;
@@ -230,10 +231,28 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
             for (int i = tid; i < D::kBins; i += kThreads) hist[i] = 0;
             __syncthreads();
         }
-        each_word([&](int, int s, uint32_t k) {
+        auto tally = [&](int s, uint32_t k) {
             const uint32_t top = k >> shift;
             if (s < len && (pass == 0 || top >> bits == prefix)) atomicAdd(&hist[top & ((1u << bits) - 1)], 1);
-        });
+        };
+        if (pass > 0) {
+            each_word([&](int, int s, uint32_t k) { tally(s, k); });
+        } else {
+            // the first pass makes the keys, and copies the slots before keep where the kept ones go to
+            // other arrays (the holes among them are filled by the moves)
+            for (int i = wa; i < wb; i += U) {
+                if (i > wa) load_words(i);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (i + u < wb) {
+                        const int s = slot_of(i + u);
+                        const uint32_t k = evict_key(x[u], p[u] >= first_recent);
+                        if (keys) keys[(i + u) * 32 + lane] = k;
+                        tally(s, k);
+                        if (a.weights_out && s < a.keep) a.weights_out[at + s] = x[u], a.positions_out[at + s] = p[u];
+                    }
+            }
+        }
         cluster_sync<C>();
         // thread t has the kPer bins from kBins - 1 - kPer t downwards
         int four[4] = {0, 0, 0, 0};
@@ -355,13 +374,12 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     each_word([&](int i, int s, uint32_t k) {
         const bool keep = s < len && (k > last_key || (k == last_key && s <= last_slot));
         const uint32_t mask = __ballot_sync(0xffffffffu, keep);
-        if (lane == 0) sm.kept[i] = mask;
-        if (a.weights_out && keep && s < a.keep) a.weights_out[at + s] = w[s], a.positions_out[at + s] = pos[s];
+        if (lane == 0) kept[i] = mask;
     });
     __syncwarp();
     int my_holes = 0, my_movers = 0;
     for (int i = wa + lane; i < wb; i += 32) {
-        const uint32_t mask = sm.kept[i], low = below(word0 + i);
+        const uint32_t mask = kept[i], low = below(word0 + i);
         my_holes += __popc(~mask & low);
         my_movers += __popc(mask & ~low);
     }
@@ -396,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     auto place_of = [&](int s) { return make_int2(s, (table[s / kCachePage] * c.kv_heads + head) * kCachePage + s % kCachePage); };
 #pragma unroll 4
     for (int i = wa; i < wb; ++i) {
-        const uint32_t mask = sm.kept[i], low = below(word0 + i), h = ~mask & low, v = mask & ~low;
+        const uint32_t mask = kept[i], low = below(word0 + i), h = ~mask & low, v = mask & ~low;
         const int s = slot_of(i);
         if (h >> lane & 1) dst[hole + __popc(h & lower)] = place_of(s);
         if (v >> lane & 1) src[mover + __popc(v & lower)] = place_of(s);
@@ -439,6 +457,9 @@ int cluster_of(const CacheView& c, int sms) {
 template <int C>
 cudaError_t launch_select(const CacheEvictArgs& a, const Lists& m, int moves_here, cudaStream_t s) {
     const CacheView& c = a.c;
+    // the largest piece's bitmap, and its keys where they fit
+    const int piece = c.max_len / 32 / C + 2, key_words = piece * 32 <= kKeysHere ? piece : 0;
+    const size_t smem = sizeof(Smem) + static_cast<size_t>(key_words ? piece * 33 : piece) * 4;
     static std::atomic<uint64_t> configured{0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -453,7 +474,7 @@ cudaError_t launch_select(const CacheEvictArgs& a, const Lists& m, int moves_her
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(c.rows) * c.kv_heads * C);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = sizeof(Smem) + (static_cast<size_t>(c.max_len) / 32 / C + 2) * 4;  // the largest piece's bitmap
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -462,7 +483,7 @@ cudaError_t launch_select(const CacheEvictArgs& a, const Lists& m, int moves_her
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, cache_evict_kernel<C>, a, m, moves_here);
+    return cudaLaunchKernelEx(&cfg, cache_evict_kernel<C>, a, m, moves_here, key_words);
 }
 
 }  // namespace
