@@ -38,6 +38,10 @@ class B200Backend:
         self.device = torch.device("cuda", device)
         self._ws = None
         self._idx = None
+        self._bf16, self._f32, self._i32 = torch.bfloat16, torch.float32, torch.int32
+        # the current stream of a device as a cudaStream_t, without the Python object around it
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
 
     def _stream(self) -> int:
         return _torch().cuda.current_stream(self.device).cuda_stream
@@ -151,33 +155,27 @@ class B200Backend:
                                     query.shape[0], key.shape[0], query.shape[1], token_pos, eps, self._stream()))
 
     # ---- bounded paged KV cache (cache.py, q3_cache_*): no counterpart in backend.hpp
+    # (checks written for the host time that they cost in every call)
 
-    def _rows(self, name: str, t, n: int, heads: int | None = None):
-        """t is a bf16 [n, heads, 128] tensor on this device whose rows are contiguous; returns its row stride."""
-        torch = _torch()
-        if t.dtype != torch.bfloat16 or t.dim() != 3 or t.device != self.device:
-            raise ValueError(f"{name} must be a bf16 [rows, heads, 128] tensor on {self.device}")
-        if t.shape[0] != n or t.shape[2] != 128 or (heads is not None and t.shape[1] != heads):
-            raise ValueError(f"{name}: shape {tuple(t.shape)} does not fit")
-        stride = t.stride()
-        if stride[2] != 1 or (stride[1] != 128 and t.shape[1] > 1):
-            raise ValueError(f"{name}: the heads of a row must be contiguous")
-        return stride[0] if n > 1 else 128 * t.shape[1]
+    def _heads(self, name: str, t, n: int, heads: int, index: int) -> int:
+        """The row stride of t, a bf16 [n, heads, 128] tensor on device `index` whose rows are contiguous."""
+        shape, stride = t.shape, t.stride()
+        if (t.dtype is not self._bf16 or len(shape) != 3 or shape[0] != n or shape[1] != heads or shape[2] != 128
+                or stride[2] != 1 or (stride[1] != 128 and heads > 1) or t.get_device() != index):
+            raise ValueError(f"{name} must be a bf16 [{n}, {heads}, 128] tensor on {self.device} with contiguous rows")
+        return stride[0] if n > 1 else 128 * heads
 
-    def _ints(self, name: str, t, n: int) -> int:
-        if t.dtype != _torch().int32 or t.device != self.device or tuple(t.shape) != (n,) or not t.is_contiguous():
+    def _ints(self, name: str, t, n: int, index: int) -> int:
+        if t.dtype is not self._i32 or t.dim() != 1 or t.numel() != n or t.get_device() != index or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 tensor of {n} on {self.device}")
         return t.data_ptr()
 
-    def _scratch(self, need: int):
-        # from torch's stream-ordered allocator at every call: calls on different streams and
-        # captured graphs never share one
-        torch = _torch()
-        return torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
-
-    def _own(self, cache):
-        if cache.device != self.device:
-            raise ValueError(f"the cache is on {cache.device}, this backend on {self.device}")
+    def _cache_call(self, cache):
+        """The library, the cache's device index and the current stream there."""
+        index = self.device.index
+        if cache.device.index != index or not cache.h:
+            raise ValueError(f"the cache is closed or on {cache.device}, this backend on {self.device}")
+        return lib(), index, self._raw_stream(index)
 
     def cache_append(self, cache, query, key, value, q_norm, k_norm, rope: RopeCache, token_pos, slots, query_out,
                      epsilon: float, lens_out=None, row_seq=None):
@@ -185,39 +183,45 @@ class B200Backend:
         be strided) is normalised and rotated as qk_norm_rope does at token_pos[i]; the query goes to query_out (may
         be query), key and value to slot slots[i] of sequence row_seq[i] (None: sequence i).  slots[i] = -1 skips
         the row.  lens_out[i] = slots[i] + 1 (may be slots)."""
-        self._own(cache)
-        torch = _torch()
+        L, index, stream = self._cache_call(cache)
         n, qh = query.shape[0], query.shape[1]
-        qs = self._rows("query", query, n)
-        ks = self._rows("key", key, n, cache.kv_heads)
-        vs = self._rows("value", value, n, cache.kv_heads)
-        os_ = self._rows("query_out", query_out, n, qh)
+        qs = self._heads("query", query, n, qh, index)
+        ks = self._heads("key", key, n, cache.kv_heads, index)
+        vs = self._heads("value", value, n, cache.kv_heads, index)
+        os_ = self._heads("query_out", query_out, n, qh, index)
+        cosine, sine = rope.cosine, rope.sine
         for t in (q_norm, k_norm):
-            if t.dtype != torch.bfloat16 or t.numel() != 128 or not t.is_contiguous() or t.device != self.device:
+            if t.dtype is not self._bf16 or t.numel() != 128 or t.get_device() != index or not t.is_contiguous():
                 raise ValueError("q_norm and k_norm must be contiguous bf16 tensors of 128")
-        for t in (rope.cosine, rope.sine):
-            if (t.dtype != torch.float32 or t.shape != rope.cosine.shape or t.shape[1] != 64 or not t.is_contiguous()
-                    or t.device != self.device):
+        for t in (cosine, sine):
+            if (t.dtype is not self._f32 or t.dim() != 2 or t.shape[1] != 64 or t.get_device() != index
+                    or not t.is_contiguous()):
                 raise ValueError("RoPE tables must be contiguous fp32 [positions, 64]")
-        check(lib().q3_cache_append(
-            cache.h, _p(query), qs, _p(key), ks, _p(value), vs, _p(q_norm), _p(k_norm), _p(rope.cosine),
-            _p(rope.sine), rope.cosine.shape[0], self._ints("token_pos", token_pos, n), self._ints("slots", slots, n),
-            None if row_seq is None else self._ints("row_seq", row_seq, n), n, qh, _p(query_out), os_,
-            None if lens_out is None else self._ints("lens_out", lens_out, n), epsilon, self._stream()))
+        if sine.shape[0] != cosine.shape[0]:
+            raise ValueError("RoPE tables differ in length")
+        status = L.q3_cache_append(
+            cache.h, query.data_ptr(), qs, key.data_ptr(), ks, value.data_ptr(), vs, q_norm.data_ptr(),
+            k_norm.data_ptr(), cosine.data_ptr(), sine.data_ptr(), cosine.shape[0],
+            self._ints("token_pos", token_pos, n, index), self._ints("slots", slots, n, index),
+            None if row_seq is None else self._ints("row_seq", row_seq, n, index), n, qh, query_out.data_ptr(), os_,
+            None if lens_out is None else self._ints("lens_out", lens_out, n, index), epsilon, stream)
+        if status:
+            check(status)
 
     def cache_attention(self, cache, query, lens, output, accumulate: bool = True):
         """output[r] = attention of query[r] (bf16 [rows, q_heads, 128], rows may be strided) over slots
         0 .. lens[r] - 1 of sequence r (q3_cache_attention); accumulate adds each slot's probabilities, summed over
         the query heads of its kv head, to cache.weights.  output may be query."""
-        self._own(cache)
-        L = lib()
-        qh = query.shape[1]
-        qs = self._rows("query", query, cache.rows)
-        os_ = self._rows("output", output, cache.rows, qh)
-        need = L.q3_cache_attention_workspace_bytes(cache.h, qh, accumulate)
-        ws = self._scratch(need)
-        check(L.q3_cache_attention(cache.h, _p(query), qs, self._ints("lens", lens, cache.rows), _p(output), os_, qh,
-                                   accumulate, _p(ws), ws.numel(), self._stream()))
+        L, index, stream = self._cache_call(cache)
+        rows, qh = cache.rows, query.shape[1]
+        qs = self._heads("query", query, rows, qh, index)
+        os_ = self._heads("output", output, rows, qh, index)
+        at = self._ints("lens", lens, rows, index)
+        ws = cache._scratch(("attention", qh, accumulate))
+        status = L.q3_cache_attention(cache.h, query.data_ptr(), qs, at, output.data_ptr(), os_, qh, accumulate,
+                                      ws.data_ptr(), ws.numel(), stream)
+        if status:
+            check(status)
 
     def cache_evict(self, cache, lens, next_pos, keep: int, recent: int, lens_out, weights_out=None,
                     positions_out=None):
@@ -225,20 +229,22 @@ class B200Backend:
         >= next_pos[r] - recent first, then the largest weights, the lower slot among equals.  In place, or weights
         and positions to weights_out and positions_out (laid out as the cache's).  lens_out[r] = min(lens[r], keep)
         (may be lens)."""
-        self._own(cache)
-        L = lib()
+        L, index, stream = self._cache_call(cache)
         for t, like in ((weights_out, cache.weights), (positions_out, cache.positions)):
-            if t is not None and (like is None or t.dtype != like.dtype or t.shape != like.shape or
-                                  t.stride() != like.stride() or t.device != self.device):
+            if t is not None and (like is None or t.dtype is not like.dtype or t.shape != like.shape or
+                                  t.stride() != like.stride() or t.get_device() != index):
                 raise ValueError("weights_out and positions_out must be laid out as the cache's")
         if keep < 1 or recent < 0:
             raise ValueError("cache_evict: keep must be at least 1 and recent at least 0")
-        ws = self._scratch(L.q3_cache_evict_workspace_bytes(cache.h, keep))
-        check(L.q3_cache_evict(cache.h, self._ints("lens", lens, cache.rows),
-                               self._ints("next_pos", next_pos, cache.rows), keep, recent,
-                               None if weights_out is None else _p(weights_out),
-                               None if positions_out is None else _p(positions_out),
-                               self._ints("lens_out", lens_out, cache.rows), _p(ws), ws.numel(), self._stream()))
+        rows = cache.rows
+        a, b, c = (self._ints(name, t, rows, index)
+                   for name, t in (("lens", lens), ("next_pos", next_pos), ("lens_out", lens_out)))
+        ws = cache._scratch(("evict", keep))
+        status = L.q3_cache_evict(cache.h, a, b, keep, recent, None if weights_out is None else weights_out.data_ptr(),
+                                  None if positions_out is None else positions_out.data_ptr(), c, ws.data_ptr(),
+                                  ws.numel(), stream)
+        if status:
+            check(status)
 
     # backend.hpp:35 -- synchronises to return the id, as the reference does
     def argmax(self, logits) -> int:

@@ -64,6 +64,7 @@ class PagedCache:
         h = C.c_void_p()
         check(lib().q3_cache_create(C.byref(d), dev.index, C.byref(h)))
         self.h = h
+        self._empty, self._uint8, self._need = torch.empty, torch.uint8, {}
         # the zeroed state is there before any stream's kernels can reach it
         torch.cuda.current_stream(dev).synchronize()
 
@@ -72,6 +73,19 @@ class PagedCache:
         if t.stride(2) != 1 or t.stride(0) != t.shape[1] * t.stride(1) or t.stride() != like.stride():
             raise ValueError("PagedCache: weights and positions must have contiguous slots and evenly spaced heads, "
                              "laid out alike")
+
+    def _scratch(self, call):
+        """A workspace for one call, ("attention", q_heads, accumulate) or ("evict", keep), from torch's
+        stream-ordered allocator: calls on different streams and captured graphs never share one."""
+        need = self._need.get(call)
+        if need is None:
+            if call[0] == "attention":
+                need = lib().q3_cache_attention_workspace_bytes(self.h, call[1], call[2])
+            else:
+                need = lib().q3_cache_evict_workspace_bytes(self.h, call[1])
+            if len(self._need) < 1024:
+                self._need[call] = need
+        return self._empty(max(need, 16), dtype=self._uint8, device=self.device)
 
     def sync(self):
         """Waits for the current stream and raises if a kernel met a value out of range in device memory."""

@@ -16,6 +16,8 @@ struct q3_cache {
     q3::CacheView view{};
     int device = 0;
     int sms = 148;
+    q3::CacheMaps maps{};  // of the pools; mapped: they have been made
+    bool mapped = false;
 };
 
 namespace q3 {
@@ -182,6 +184,7 @@ int q3_cache_create(const q3_cache_desc* d, int device, q3_cache** out) {
     v.err = d->state_dev;
     v.next_chunk = d->state_dev + 1;
     v.arrived = d->state_dev + 2;
+    c->mapped = cache_maps(v, &c->maps);
     *out = c;
     return Q3_OK;
 }
@@ -281,6 +284,7 @@ int q3_cache_attention(q3_cache* c, const uint16_t* q, size_t q_stride, const in
              "q3_cache_attention: workspace missing, too small or not 16-byte aligned");
     DeviceScope scope(c->device);
     Q3_CUDA(scope.status);
+    if (!c->mapped) return fail(Q3_ERR_CUDA, "q3_cache_attention: no tensor maps of the pages (no CUDA driver?)");
     CacheAttnArgs a{};
     a.c = w;
     a.q = reinterpret_cast<const bf16*>(q);
@@ -291,7 +295,7 @@ int q3_cache_attention(q3_cache* c, const uint16_t* q, size_t q_stride, const in
     a.q_heads = static_cast<int>(q_heads);
     a.accumulate = accumulate != 0;
     a.ws = ws;
-    return launched(launch_cache_attention(a, c->sms, static_cast<cudaStream_t>(stream)), "q3_cache_attention");
+    return launched(launch_cache_attention(a, c->maps, c->sms, static_cast<cudaStream_t>(stream)), "q3_cache_attention");
 }
 
 size_t q3_cache_evict_workspace_bytes(const q3_cache* c, size_t keep) {

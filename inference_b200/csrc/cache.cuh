@@ -58,8 +58,14 @@ struct CacheAttnArgs {
     int q_heads, accumulate;
     void* ws;
 };
+// Tensor maps of the K and V pools as [num_pages x kv_heads x 64, 128] matrices:
+// boxes of 64 columns by 64 rows (a full tile's half) and by 16.
+struct CacheMaps {
+    CUtensorMap k64, v64, k16, v16;
+};
+bool cache_maps(const CacheView& c, CacheMaps* maps);  // false without a driver
 size_t cache_attention_ws_bytes(const CacheView& c, int q_heads, int accumulate, int sms);
-cudaError_t launch_cache_attention(const CacheAttnArgs& a, int sms, cudaStream_t s);
+cudaError_t launch_cache_attention(const CacheAttnArgs& a, const CacheMaps& maps, int sms, cudaStream_t s);
 
 struct CacheEvictArgs {
     CacheView c;

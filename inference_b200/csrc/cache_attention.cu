@@ -131,15 +131,9 @@ __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, int 
         : "memory");
 }
 
-// Tensor maps of the K and V pools as [num_pages x kv_heads x 64, 128] matrices:
-// boxes of 64 columns by 64 rows (a full tile's half) and by 16.
-struct Maps {
-    CUtensorMap k64, v64, k16, v16;
-};
-
 template <int NT>
 __global__ void __maxnreg__(NT == 1 ? 128 : 168)
-    cache_attention_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ Maps maps,
+    cache_attention_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ CacheMaps maps,
                            const __grid_constant__ Parts parts) {
     using C = Cfg<NT>;
     constexpr int S = C::kStages;
@@ -744,7 +738,7 @@ static_assert(2 * (sizeof(Smem<1>) + 1024 + 1024) <= 228 * 1024, "two CTAs must 
 static_assert(2 * (sizeof(Smem<2>) + 1024 + 1024) <= 228 * 1024, "two CTAs must share an SM");
 
 template <int NT>
-cudaError_t launch_nt(const CacheAttnArgs& a, const Maps& maps, const Parts& parts, cudaStream_t s) {
+cudaError_t launch_nt(const CacheAttnArgs& a, const CacheMaps& maps, const Parts& parts, cudaStream_t s) {
     // the shared-memory opt-in once per device (not per launch: launches may be captured)
     static std::atomic<uint64_t> configured{0};
     int dev = 0;
@@ -768,13 +762,14 @@ size_t cache_attention_ws_bytes(const CacheView& c, int q_heads, int accumulate,
     return layout(c, q_heads, accumulate, sms, nullptr, &p);
 }
 
-cudaError_t launch_cache_attention(const CacheAttnArgs& a, int sms, cudaStream_t s) {
-    const CacheView& c = a.c;
-    Maps maps;
+bool cache_maps(const CacheView& c, CacheMaps* maps) {
     const long long rows = static_cast<long long>(c.num_pages) * c.kv_heads * kCachePage;
-    if (!make_map(&maps.k64, c.k, rows, 64) || !make_map(&maps.v64, c.v, rows, 64) ||
-        !make_map(&maps.k16, c.k, rows, 16) || !make_map(&maps.v16, c.v, rows, 16))
-        return cudaErrorInvalidValue;
+    return make_map(&maps->k64, c.k, rows, 64) && make_map(&maps->v64, c.v, rows, 64) &&
+           make_map(&maps->k16, c.k, rows, 16) && make_map(&maps->v16, c.v, rows, 16);
+}
+
+cudaError_t launch_cache_attention(const CacheAttnArgs& a, const CacheMaps& maps, int sms, cudaStream_t s) {
+    const CacheView& c = a.c;
     Parts parts;
     layout(c, a.q_heads, a.accumulate, sms, static_cast<uint8_t*>(a.ws), &parts);
     cudaError_t e = a.q_heads / c.kv_heads <= 8 ? launch_nt<1>(a, maps, parts, s) : launch_nt<2>(a, maps, parts, s);
