@@ -32,6 +32,8 @@ constexpr int kAppendWarps = 8;
 __global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const CacheAppendArgs a) {
     const CacheView& c = a.c;
     const int i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_trigger();
     const int slot = a.slots[i];
     const int pos = a.token_pos[i];
     const int seq = a.row_seq ? a.row_seq[i] : i;
@@ -129,8 +131,7 @@ int launched(cudaError_t e, const char* what) {
 }  // namespace
 
 cudaError_t launch_cache_append(const CacheAppendArgs& a, cudaStream_t s) {
-    cache_append_kernel<<<a.n, kAppendWarps * 32, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch_after(cache_append_kernel, dim3(a.n), kAppendWarps * 32, 0, s, a);
 }
 
 }  // namespace q3

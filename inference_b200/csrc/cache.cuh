@@ -32,6 +32,25 @@ __device__ __forceinline__ size_t cache_kv_offset(const CacheView& c, int page, 
     return ((static_cast<size_t>(page) * c.kv_heads + head) * kCachePage + slot % kCachePage) * kCacheHd;
 }
 
+// Launches behind the stream's previous kernel by programmatic dependent launch: the
+// kernel's CTAs may become resident while that one ends, and wait for its end and its
+// writes (pdl_wait) before they read or write any of the caller's memory.  Every kernel
+// triggers its own dependents after that wait.
+template <class Kernel, class... Args>
+cudaError_t launch_after(Kernel kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 struct CacheAppendArgs {
     CacheView c;
     const bf16 *q, *k, *v;

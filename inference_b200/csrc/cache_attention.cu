@@ -142,7 +142,6 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
     const CacheView& c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.q_heads / c.kv_heads;
-    pdl_trigger();  // the joining kernel may set itself up; it waits for this one's end
     if (tid == kConsumers) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&sm.full[s], 1);
@@ -154,6 +153,8 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
         prefetch_map(&maps.k16);
         prefetch_map(&maps.v16);
     }
+    pdl_wait();     // what ran before may have written the lengths, queries and pages
+    pdl_trigger();  // the joining kernel may set itself up; it waits for this one's end
     scan_rows<kThreads>(a.lens, c, sm.before, sm.scan);
 
     if (warp == kWarps) {
@@ -569,6 +570,7 @@ __global__ void __maxnreg__(64)
     };
     if (t0 < t1) look_up(t0);
     pdl_wait();
+    pdl_trigger();
     if (me == 0 && tid == 0) *c.next_chunk = 0;  // for the cache's next attention
 
     // heads side by side in a warp: the power of two that holds G
@@ -751,8 +753,7 @@ cudaError_t launch_nt(const CacheAttnArgs& a, const CacheMaps& maps, const Parts
         if (e != cudaSuccess) return e;
         configured.fetch_or(bit);
     }
-    cache_attention_kernel<NT><<<parts.workers, kThreads, sizeof(Smem<NT>) + 1024, s>>>(a, maps, parts);
-    return cudaGetLastError();
+    return launch_after(cache_attention_kernel<NT>, dim3(parts.workers), kThreads, sizeof(Smem<NT>) + 1024, s, a, maps, parts);
 }
 
 }  // namespace
@@ -774,16 +775,7 @@ cudaError_t launch_cache_attention(const CacheAttnArgs& a, const CacheMaps& maps
     layout(c, a.q_heads, a.accumulate, sms, static_cast<uint8_t*>(a.ws), &parts);
     cudaError_t e = a.q_heads / c.kv_heads <= 8 ? launch_nt<1>(a, maps, parts, s) : launch_nt<2>(a, maps, parts, s);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(parts.workers);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, cache_join_kernel, a, parts);
+    return launch_after(cache_join_kernel, dim3(parts.workers), kJoinThreads, 0, s, a, parts);
 }
 
 }  // namespace q3

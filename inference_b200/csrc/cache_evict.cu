@@ -136,6 +136,8 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     const CacheView& c = a.c;
     const int rh = blockIdx.x / C, rank = blockIdx.x % C, row = rh / c.kv_heads, head = rh % c.kv_heads;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_wait();
+    pdl_trigger();
     const int len = a.lens[row];
     const int first_recent =
         static_cast<int>(max(static_cast<long long>(a.next_pos[row]) - a.recent, static_cast<long long>(INT_MIN)));
@@ -143,7 +145,6 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     const size_t at = cache_slot_index(c, row, head);
     const float* w = c.weights + at;
     const int32_t* pos = c.positions + at;
-    if (!moves_here) pdl_trigger();
     using D = Digits<C>;
     for (int i = tid; i < D::kBins; i += kThreads) sm.hist[0][i] = 0;
     if (tid == 0) sm.n_mine = 0;
@@ -435,6 +436,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
 __global__ void __launch_bounds__(kMoveThreads, 4) cache_evict_move_kernel(const CacheEvictArgs a, const Lists m, int chunks) {
     const int rh = blockIdx.x / chunks, first = blockIdx.x % chunks * kMoveChunk;
     pdl_wait();
+    pdl_trigger();
     const int n = min(m.count[rh], first + kMoveChunk);
     const size_t list = static_cast<size_t>(rh) * m.cap;
     move_slots(a, m.dst + list, m.src + list, static_cast<size_t>(rh) * a.c.slot_stride, first + (threadIdx.x >> 4),
@@ -476,13 +478,15 @@ cudaError_t launch_select(const CacheEvictArgs& a, const Lists& m, int moves_her
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = C;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // as launch_after
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = C;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = C > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, cache_evict_kernel<C>, a, m, moves_here, key_words);
 }
 
@@ -513,16 +517,7 @@ cudaError_t launch_cache_evict(const CacheEvictArgs& a, int sms, cudaStream_t s)
     }
     if (e != cudaSuccess || moves_here) return e;
     const int chunks = (m.cap + kMoveChunk - 1) / kMoveChunk;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(rh) * chunks);
-    cfg.blockDim = dim3(kMoveThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, cache_evict_move_kernel, a, m, chunks);
+    return launch_after(cache_evict_move_kernel, dim3(static_cast<unsigned>(rh) * chunks), kMoveThreads, 0, s, a, m, chunks);
 }
 
 }  // namespace q3
