@@ -472,7 +472,7 @@ constexpr int kJoinTiles = 64;  // tiles whose runs are looked up at a time, a t
 constexpr int kJoinRuns = 8;    // runs joined between two barriers
 struct JoinSmem {
     int4 where[kJoinTiles];                      // of a run met: row, head, first tile here, slots here
-    int4 span[kJoinTiles];                       // its first tile of all, its tiles, first and last chunk's place
+    int4 span[kJoinTiles];                       // its first tile of all, first and last chunk's place; units first << 16 | last
     float2 part[kJoinRuns][kJoinWarps][16];      // each warp's maximum and sum
     float2 ml[kJoinRuns][16];                    // maximum, 1 / sum (0: a bad page, no weights)
     int before[kJoinThreads + 1];
@@ -523,16 +523,6 @@ __device__ __forceinline__ void add_weights(float* w, const float* s, const floa
     }
 }
 
-// Maximum and sum of two parts, in this order.  An infinite maximum with the sum 0 marks
-// a bad page (no scores give it: the sum to an infinite maximum is NaN) and spreads.
-__device__ __forceinline__ bool bad_page(float2 v) { return v.x == INFINITY && v.y == 0.f; }
-__device__ __forceinline__ float2 join_ml(float2 x, float2 y) {
-    if (bad_page(x)) return x;
-    if (bad_page(y)) return y;
-    const float m = fmaxf(x.x, y.x), base = m == -INFINITY ? 0.f : m;
-    return make_float2(m, x.y * exp2f(x.x - base) + y.y * exp2f(y.x - base));
-}
-
 __global__ void __maxnreg__(64)
     cache_join_kernel(const __grid_constant__ CacheAttnArgs a, const __grid_constant__ Parts parts) {
     __shared__ JoinSmem sm;
@@ -564,7 +554,14 @@ __global__ void __maxnreg__(64)
             const int at = __popc(sm.starts[warp] & ((1u << lane) - 1)) + (warp ? __popc(sm.starts[0]) : 0);
             const int run0 = t + tid - p.tile, here = min(n - tid, p.tiles - p.tile);
             sm.where[at] = make_int4(p.row, p.head, p.tile, min(here * kCachePage, p.len - p.tile * kCachePage));
-            sm.span[at] = make_int4(run0, p.tiles, plan_place_of(plan, run0), plan_place_of(plan, run0 + p.tiles - 1));
+            const int c0 = plan_place_of(plan, run0), c1 = plan_place_of(plan, run0 + p.tiles - 1);
+            int slice = 0;  // of the run's outputs, in units of 4 dims
+            if (c0 != c1 && max(run0, t0) == t + tid) {  // cut, and not met before in this share
+                const int first = equal_share_of(mine, run0);
+                const Equal part = equal_make(G * kCacheHd / 4, equal_share_of(mine, run0 + p.tiles - 1) - first + 1);
+                slice = equal_first(part, me - first) << 16 | equal_first(part, me - first + 1);
+            }
+            sm.span[at] = make_int4(run0, c0, c1, slice);
         }
         __syncthreads();
     };
@@ -581,10 +578,11 @@ __global__ void __maxnreg__(64)
             const int nr = min(kJoinRuns, runs - r0);
             // ---- maximum and sum; thread: head tid % wide of every (threads / wide)-th part
             for (int r = 0; r < nr; ++r) {
-                const int c0 = sm.span[r0 + r].z, c1 = sm.span[r0 + r].w;
+                const int c0 = sm.span[r0 + r].y, c1 = sm.span[r0 + r].z;
                 if (c0 == c1) continue;
                 const int h = tid % wide, deal = kJoinThreads / wide;
-                float2 v = make_float2(-INFINITY, 0.f);
+                float m = -INFINITY, l = 0.f;
+                bool bad = false;
                 if (h < G)
                     for (int s0 = c0 + tid / wide; s0 <= c1; s0 += 8 * deal) {
                         float2 x[8];
@@ -595,39 +593,46 @@ __global__ void __maxnreg__(64)
                             x[u] = s <= c1 ? parts.pml[static_cast<size_t>(s * 2 + (s == c0)) * G + h]
                                            : make_float2(-INFINITY, 0.f);
                         }
-                        float m = v.x;
-                        bool bad = bad_page(v);
+                        const float before = m;
 #pragma unroll
                         for (int u = 0; u < 8; ++u) {
-                            bad = bad || bad_page(x[u]);
+                            bad = bad || (x[u].x == INFINITY && x[u].y == 0.f);  // a bad page: see the parts
                             m = fmaxf(m, x[u].x);
                         }
                         const float base = m == -INFINITY ? 0.f : m;
-                        float l = v.y * exp2f(v.x - base);
+                        l *= exp2f(before - base);
 #pragma unroll
                         for (int u = 0; u < 8; ++u) l += x[u].y * exp2f(x[u].x - base);
-                        v = bad ? make_float2(INFINITY, 0.f) : make_float2(m, l);
                     }
-                for (int off = wide; off < 32; off <<= 1) {
-                    const float2 w =
-                        make_float2(__shfl_xor_sync(0xffffffffu, v.x, off), __shfl_xor_sync(0xffffffffu, v.y, off));
-                    v = (lane & off) ? join_ml(w, v) : join_ml(v, w);  // the same order on both sides
-                }
-                if (lane < wide) sm.part[r][warp][lane] = v;
+                float M = m;
+                for (int off = wide; off < 32; off <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+                l *= exp2f(m - (M == -INFINITY ? 0.f : M));
+                for (int off = wide; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+                bad = __any_sync(0xffffffffu, bad);
+                if (lane < wide) sm.part[r][warp][lane] = make_float2(bad ? INFINITY : M, bad ? 0.f : l);
             }
             __syncthreads();
             {
                 const int r = tid >> 4, h = tid & 15;
                 if (r < nr && h < G) {
                     const int4 w = sm.where[r0 + r], sp = sm.span[r0 + r];
-                    if (sp.z == sp.w) {
+                    if (sp.y == sp.z) {
                         if (a.accumulate)
                             sm.ml[r][h] = parts.ml[static_cast<size_t>(w.x) * a.q_heads + w.y * G + h];
                     } else {
-                        float2 v = sm.part[r][0][h];
+                        float2 x[kJoinWarps];
+                        float M = -INFINITY, L = 0.f;
+                        bool bad = false;
 #pragma unroll
-                        for (int i = 1; i < kJoinWarps; ++i) v = join_ml(v, sm.part[r][i][h]);
-                        sm.ml[r][h] = make_float2(v.x == -INFINITY ? 0.f : v.x, bad_page(v) ? 0.f : 1.f / v.y);
+                        for (int i = 0; i < kJoinWarps; ++i) {
+                            x[i] = sm.part[r][i][h];
+                            bad = bad || (x[i].x == INFINITY && x[i].y == 0.f);
+                            M = fmaxf(M, x[i].x);
+                        }
+                        const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+                        for (int i = 0; i < kJoinWarps; ++i) L += x[i].y * exp2f(x[i].x - base);
+                        sm.ml[r][h] = make_float2(base, bad ? 0.f : 1.f / L);
                     }
                 }
             }
@@ -635,11 +640,7 @@ __global__ void __maxnreg__(64)
             // ---- outputs of cut runs, in units of 4 dims: a warp takes units, its lanes their parts
             for (int r = 0; r < nr; ++r) {
                 const int4 w = sm.where[r0 + r], sp = sm.span[r0 + r];
-                if (sp.z == sp.w || max(sp.x, t0) != sp.x + w.z) continue;  // whole, or met before in this share
-                const int first = equal_share_of(mine, sp.x), units = G * kCacheHd / 4;
-                const Equal slice = equal_make(units, equal_share_of(mine, sp.x + sp.y - 1) - first + 1);
-                const int u0 = equal_first(slice, me - first), u1 = equal_first(slice, me - first + 1);
-                const int P = sp.w - sp.z + 1;
+                const int u0 = sp.w >> 16, u1 = sp.w & 0xFFFF, c0 = sp.y, c1 = sp.z, P = c1 - c0 + 1;
                 const int turns = P <= 2 ? 2 : P <= 4 ? 4 : P <= 8 ? 8 : P <= 16 ? 16 : 32;
                 const int width = 32 / turns, turn = lane / width;
                 for (int u = u0 + warp * width; u < u1; u += kJoinWarps * width) {
@@ -648,8 +649,8 @@ __global__ void __maxnreg__(64)
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (unit < u1)
 #pragma unroll 4
-                        for (int s = sp.z + turn; s <= sp.w; s += turns) {
-                            const size_t at = static_cast<size_t>(s * 2 + (s == sp.z)) * G + h;
+                        for (int s = c0 + turn; s <= c1; s += turns) {
+                            const size_t at = static_cast<size_t>(s * 2 + (s == c0)) * G + h;
                             const float f = exp2f(parts.pml[at].x - ml.x);
                             const float4 v = reinterpret_cast<const float4*>(parts.po + at * kCacheHd)[unit % (kCacheHd / 4)];
                             x.x += v.x * f, x.y += v.y * f, x.z += v.z * f, x.w += v.w * f;
@@ -775,7 +776,10 @@ cudaError_t launch_cache_attention(const CacheAttnArgs& a, const CacheMaps& maps
     layout(c, a.q_heads, a.accumulate, sms, static_cast<uint8_t*>(a.ws), &parts);
     cudaError_t e = a.q_heads / c.kv_heads <= 8 ? launch_nt<1>(a, maps, parts, s) : launch_nt<2>(a, maps, parts, s);
     if (e != cudaSuccess) return e;
-    return launch_after(cache_join_kernel, dim3(parts.workers), kJoinThreads, 0, s, a, parts);
+    // two CTAs an SM are resident beside the first kernel's; with 8 tiles a worker or more the work is worth
+    // eight, though the others start (and look up their runs) only when that one ends
+    const int join_ctas = max_tiles(c) >= 8 * static_cast<size_t>(parts.workers) ? 4 * parts.workers : parts.workers;
+    return launch_after(cache_join_kernel, dim3(join_ctas), kJoinThreads, 0, s, a, parts);
 }
 
 }  // namespace q3
