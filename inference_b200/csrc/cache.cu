@@ -6,6 +6,8 @@
 // query and key are rotated to its position, its K/V go to any slot, and the
 // slots a sequence attends to can be cut to a budget (cache_evict.cu) by the
 // attention they have received (cache_attention.cu).
+#include <algorithm>
+#include <atomic>
 #include <climits>
 #include <new>
 
@@ -23,74 +25,291 @@ struct q3_cache {
 namespace q3 {
 namespace {
 
-constexpr int kAppendWarps = 8;
+constexpr int kAppendWarps = 16;    // most warps a row (few rows); consumer warps (many)
+constexpr int kAppendStages = 16;   // most rows in flight a CTA
+constexpr int kAppendRing = 200 * 1024;
 
-// One CTA per new token, one head per warp and turn.  A head is a 256-byte row:
-// lane l holds dims l, l + 32, l + 64, l + 96, so that a rotation's two halves
-// (i and i + 64) sit in one lane; RMSNorm and RoPE as qk_norm_rope
-// (cuda/kernels/qk_norm_rope.cuh:14-90): fp32 throughout, one rounding.
-__global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const CacheAppendArgs a) {
+// Two fp32 values in a 64-bit register, and the packed arithmetic on them (each
+// element rounded as the scalar operation rounds it).
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+    f32x2 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ f32x2 pair(uint32_t bf) { return pair(bf_lo(bf), bf_hi(bf)); }  // of two BF16
+__device__ __forceinline__ f32x2 mul2(f32x2 x, f32x2 y) {
+    f32x2 v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 x, f32x2 y, f32x2 z) {
+    f32x2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+    return v;
+}
+__device__ __forceinline__ float2 unpair(f32x2 v) {
+    float2 x;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x.x), "=f"(x.y) : "l"(v));
+    return x;
+}
+__device__ __forceinline__ uint32_t to_bf2(f32x2 v) {
+    const float2 x = unpair(v);
+    const __nv_bfloat162 b = __floats2bfloat162_rn(x.x, x.y);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// A unit is four heads of one kind (queries, keys or values), eight lanes each: lane j
+// holds dims 8 j .. 8 j + 7 and 64 + 8 j .. of its head, so that both halves of a
+// rotation sit in one lane.  RMSNorm and RoPE as qk_norm_rope
+// (cuda/kernels/qk_norm_rope.cuh:14-90): fp32 throughout, one rounding; the norm's
+// weights are multiplied into the rotation once for all of a row's heads, and the
+// arithmetic runs on pairs.
+struct Rotation {
+    // (a, b), the halves of a pair of dims -> (a (w0 c) - b (w1 s), b (w1 c) + a (w0 s)), times the norm's scale
+    f32x2 ac[4], as[4], bc[4], bs[4];
+    __device__ __forceinline__ void make(uint4 n0, uint4 n1, const float* cos_row, const float* sin_row, int sub) {
+        const uint32_t w0[4] = {n0.x, n0.y, n0.z, n0.w}, w1[4] = {n1.x, n1.y, n1.z, n1.w};
+        float4 c[2], s[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            c[j] = reinterpret_cast<const float4*>(cos_row)[2 * sub + j];
+            s[j] = reinterpret_cast<const float4*>(sin_row)[2 * sub + j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x2 c2 = j & 1 ? pair(c[j / 2].z, c[j / 2].w) : pair(c[j / 2].x, c[j / 2].y);
+            const f32x2 s2 = j & 1 ? pair(s[j / 2].z, s[j / 2].w) : pair(s[j / 2].x, s[j / 2].y);
+            ac[j] = mul2(pair(w0[j]), c2);
+            as[j] = mul2(pair(w0[j]), s2);
+            bc[j] = mul2(pair(w1[j]), c2);
+            bs[j] = mul2(pair(w1[j]), mul2(s2, pair(-1.f, -1.f)));
+        }
+    }
+    // one head by its eight lanes, four heads a warp
+    __device__ __forceinline__ void apply(uint4& x, uint4& y, float eps) const {
+        const uint32_t w0[4] = {x.x, x.y, x.z, x.w}, w1[4] = {y.x, y.y, y.z, y.w};
+        f32x2 s2 = pair(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s2 = fma2(pair(w1[j]), pair(w1[j]), fma2(pair(w0[j]), pair(w0[j]), s2));
+        float ss = unpair(s2).x + unpair(s2).y;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float scale = 1.0f / sqrtf(ss / 128.0f + eps);
+        const f32x2 scale2 = pair(scale, scale);
+        uint32_t r0[4], r1[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x2 a2 = pair(w0[j]), b2 = pair(w1[j]);
+            r0[j] = to_bf2(mul2(fma2(b2, bs[j], mul2(a2, ac[j])), scale2));
+            r1[j] = to_bf2(mul2(fma2(a2, as[j], mul2(b2, bc[j])), scale2));
+        }
+        x = make_uint4(r0[0], r0[1], r0[2], r0[3]);
+        y = make_uint4(r1[0], r1[1], r1[2], r1[3]);
+    }
+};
+
+// A new token's row, looked up: DEV_OK, or why it is left out.
+__device__ __forceinline__ uint32_t append_check(const CacheAppendArgs& a, int slot, int pos, int seq) {
+    if (slot < 0 || slot >= a.c.max_len) return DEV_BAD_SLOT;
+    if (pos < 0 || pos >= a.max_pos) return DEV_BAD_POSITION;
+    if (seq < 0 || seq >= a.c.rows) return DEV_BAD_SEQUENCE;
+    return DEV_OK;
+}
+__device__ __forceinline__ bool append_page_bad(const CacheView& c, int page) { return page < 0 || page >= c.num_pages; }
+__device__ __forceinline__ void append_state(const CacheView& c, int seq, int slot, int pos, int lane) {
+    if (!c.weights) return;
+    for (int h = lane; h < c.kv_heads; h += 32) {
+        const size_t at = cache_slot_index(c, seq, h) + slot;
+        c.weights[at] = 0.0f;
+        c.positions[at] = pos;
+    }
+}
+
+// Few rows: one CTA a row, its units dealt to the warps, in the order queries, keys,
+// values.  Bound: latency.
+__global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const __grid_constant__ CacheAppendArgs a) {
     const CacheView& c = a.c;
-    const int i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7;
     pdl_wait();
     pdl_trigger();
-    const int slot = a.slots[i];
-    const int pos = a.token_pos[i];
-    const int seq = a.row_seq ? a.row_seq[i] : i;
+    const int slot = a.slots[i], pos = a.token_pos[i], seq = a.row_seq ? a.row_seq[i] : i;
     if (slot == -1) return;
-    uint32_t bad = 0;
-    int page = 0;
-    if (slot < 0 || slot >= c.max_len)
-        bad = DEV_BAD_SLOT;
-    else if (pos < 0 || pos >= a.max_pos)
-        bad = DEV_BAD_POSITION;
-    else if (seq < 0 || seq >= c.rows)
-        bad = DEV_BAD_SEQUENCE;
-    else {
-        page = c.tables[seq * c.table_stride + slot / kCachePage];
-        if (page < 0 || page >= c.num_pages) bad = DEV_BAD_PAGE;
-    }
+    uint32_t bad = append_check(a, slot, pos, seq);
+    const int page = bad ? 0 : c.tables[seq * c.table_stride + slot / kCachePage];
+    if (!bad && append_page_bad(c, page)) bad = DEV_BAD_PAGE;
     if (bad) {
         if (threadIdx.x == 0) record_error(c.err, bad);
         return;
     }
-    float cs[2], sn[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        cs[j] = a.rope_cos[static_cast<size_t>(pos) * 64 + lane + 32 * j];
-        sn[j] = a.rope_sin[static_cast<size_t>(pos) * 64 + lane + 32 * j];
-    }
-    for (int h = warp; h < a.q_heads + c.kv_heads; h += kAppendWarps) {
-        const bool is_q = h < a.q_heads;
-        const int kh = h - a.q_heads;
-        const bf16* src = is_q ? a.q + i * a.q_stride + h * kCacheHd : a.k + i * a.k_stride + kh * kCacheHd;
-        const bf16* w = is_q ? a.q_norm : a.k_norm;
-        float x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = bf2f(src[lane + 32 * j]);
-        const float ss = warp_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
-        const float scale = 1.0f / sqrtf(ss / 128.0f + a.eps);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = x[j] * bf2f(w[lane + 32 * j]) * scale;
-        bf16* dst = is_q ? a.q_out + i * a.q_out_stride + h * kCacheHd : c.k + cache_kv_offset(c, page, kh, slot);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            dst[lane + 32 * j] = f2bf(x[j] * cs[j] - x[j + 2] * sn[j]);
-            dst[lane + 32 * j + 64] = f2bf(x[j + 2] * cs[j] + x[j] * sn[j]);
+    const int q_units = (a.q_heads + 3) / 4, kv_units = (c.kv_heads + 3) / 4;
+    for (int u = warp; u < q_units + 2 * kv_units; u += blockDim.x / 32) {
+        const bool is_q = u < q_units, is_k = !is_q && u < q_units + kv_units;
+        const int h = 4 * (is_q ? u : is_k ? u - q_units : u - q_units - kv_units) + (lane >> 3);
+        const bf16* src = is_q ? a.q + i * a.q_stride : is_k ? a.k + i * a.k_stride : a.v + i * a.v_stride;
+        const bool live = h < (is_q ? a.q_heads : c.kv_heads);
+        uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
+        if (live) {
+            x = reinterpret_cast<const uint4*>(src + h * kCacheHd)[sub];
+            y = reinterpret_cast<const uint4*>(src + h * kCacheHd)[sub + 8];
         }
-        if (!is_q) {
-            const uint2* from = reinterpret_cast<const uint2*>(a.v + i * a.v_stride + kh * kCacheHd);
-            reinterpret_cast<uint2*>(c.v + cache_kv_offset(c, page, kh, slot))[lane] = from[lane];
-            if (c.weights && lane == 0) {
-                const size_t at = cache_slot_index(c, seq, kh) + slot;
-                c.weights[at] = 0.0f;
-                c.positions[at] = pos;
-            }
+        if (is_q || is_k) {
+            const uint4* norm = reinterpret_cast<const uint4*>(is_q ? a.q_norm : a.k_norm);
+            Rotation turn;
+            turn.make(norm[sub], norm[sub + 8], a.rope_cos + static_cast<size_t>(pos) * 64,
+                      a.rope_sin + static_cast<size_t>(pos) * 64, sub);
+            turn.apply(x, y, a.eps);
+        }
+        if (live) {
+            uint4* to = reinterpret_cast<uint4*>(is_q ? a.q_out + i * a.q_out_stride + h * kCacheHd
+                                                      : (is_k ? c.k : c.v) + cache_kv_offset(c, page, h, slot));
+            to[sub] = x;
+            to[sub + 8] = y;
         }
     }
-    // every warp has read slots[i] (lens_out may be the same array)
+    if (warp == 0) append_state(c, seq, slot, pos, lane);
+    // every thread has read slots[i] (lens_out may be the same array)
     __syncthreads();
     if (a.lens_out && threadIdx.x == 0) a.lens_out[i] = slot + 1;
+}
+
+// Many rows: a CTA an SM streams its rows (heads, and the position's cosines and sines)
+// through a shared-memory ring by bulk copies, so that up to 200 KB an SM are in flight
+// whatever the rows' look-ups wait for; 16 warps turn the heads and write them.  Bound:
+// HBM.
+struct AppendSmem {
+    int4 row[kAppendStages];  // row (-1: the end), sequence, slot, position
+    int page[kAppendStages];
+    uint64_t full[kAppendStages], empty[kAppendStages];
+};
+
+__global__ void __launch_bounds__(kAppendWarps * 32 + 32, 1)
+    cache_append_stream_kernel(const __grid_constant__ CacheAppendArgs a, int stages, int stage_bytes) {
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ AppendSmem sm;
+    const CacheView& c = a.c;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(&sm.full[s], 1);
+            mbar_init(&sm.empty[s], kAppendWarps);
+        }
+        fence_barrier_init();
+    }
+    pdl_wait();
+    pdl_trigger();
+    __syncthreads();
+    const int q_bytes = a.q_heads * kCacheHd * 2, kv_bytes = c.kv_heads * kCacheHd * 2;
+
+    if (warp == kAppendWarps) {
+        // ---- producer: lane j looks up the CTA's row j of every 32
+        const uint64_t pol = policy_evict_first();
+        int k = 0, s = 0;
+        uint32_t round = 0;  // of the ring: stage s has been used `round` times
+        bool ok = true;
+        auto stage_free = [&]() {
+            return round == 0 || mbar_wait(&sm.empty[s], (round - 1) & 1, c.err, DEV_TMA_WAIT_TIMEOUT);
+        };
+        auto advance = [&]() {
+            ++k;
+            if (++s == stages) s = 0, ++round;
+        };
+        const int step = gridDim.x;
+        for (int i0 = blockIdx.x; i0 < a.n && ok; i0 += 32 * step) {
+            const int i = i0 + lane * step;
+            int4 row = make_int4(i, 0, -1, 0);
+            int page = 0;
+            if (i < a.n) {
+                row.z = a.slots[i];
+                row.w = a.token_pos[i];
+                row.y = a.row_seq ? a.row_seq[i] : i;
+                if (row.z != -1) {
+                    uint32_t bad = append_check(a, row.z, row.w, row.y);
+                    if (!bad) {
+                        page = c.tables[row.y * c.table_stride + row.z / kCachePage];
+                        if (append_page_bad(c, page)) bad = DEV_BAD_PAGE;
+                    }
+                    if (bad) {
+                        record_error(c.err, bad);
+                        row.z = -1;
+                    }
+                }
+            }
+            for (int j = 0; j < 32 && ok; ++j) {
+                const int4 r = make_int4(__shfl_sync(0xffffffffu, row.x, j), __shfl_sync(0xffffffffu, row.y, j),
+                                         __shfl_sync(0xffffffffu, row.z, j), __shfl_sync(0xffffffffu, row.w, j));
+                const int pg = __shfl_sync(0xffffffffu, page, j);
+                if (r.z < 0) continue;  // left out, or no such row
+                if (lane == 0) {
+                    ok = stage_free();
+                    if (ok) {
+                        uint8_t* st = ring + static_cast<size_t>(s) * stage_bytes;
+                        sm.row[s] = r;
+                        sm.page[s] = pg;
+                        mbar_arrive_expect_tx(&sm.full[s], q_bytes + 2 * kv_bytes + 512);
+                        bulk_g2s(st, a.q + r.x * a.q_stride, q_bytes, &sm.full[s], pol);
+                        bulk_g2s(st + q_bytes, a.k + r.x * a.k_stride, kv_bytes, &sm.full[s], pol);
+                        bulk_g2s(st + q_bytes + kv_bytes, a.v + r.x * a.v_stride, kv_bytes, &sm.full[s], pol);
+                        st += q_bytes + 2 * kv_bytes;
+                        bulk_g2s(st, a.rope_cos + static_cast<size_t>(r.w) * 64, 256, &sm.full[s], pol);
+                        bulk_g2s(st + 256, a.rope_sin + static_cast<size_t>(r.w) * 64, 256, &sm.full[s], pol);
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (ok) advance();
+            }
+        }
+        if (lane == 0) {
+            ok = ok && stage_free();
+            if (ok) {
+                sm.row[s].x = -1;
+                mbar_arrive(&sm.full[s]);
+            } else {
+                // a wait ran out: leave no copy in flight behind
+                for (int i = max(0, k - stages); i < k; ++i)
+                    mbar_wait(&sm.full[i % stages], (i / stages) & 1, nullptr, 0);
+            }
+        }
+        return;
+    }
+
+    const uint4 qn0 = reinterpret_cast<const uint4*>(a.q_norm)[sub], qn1 = reinterpret_cast<const uint4*>(a.q_norm)[sub + 8];
+    const uint4 kn0 = reinterpret_cast<const uint4*>(a.k_norm)[sub], kn1 = reinterpret_cast<const uint4*>(a.k_norm)[sub + 8];
+    const int q_units = (a.q_heads + 3) / 4, kv_units = (c.kv_heads + 3) / 4;
+    for (int s = 0, round = 0;;) {
+        if (!mbar_wait(&sm.full[s], round & 1, c.err, DEV_TMA_WAIT_TIMEOUT)) return;
+        const int4 r = sm.row[s];
+        if (r.x < 0) return;
+        const int page = sm.page[s];
+        const uint8_t* st = ring + static_cast<size_t>(s) * stage_bytes;
+        const float* cos_row = reinterpret_cast<const float*>(st + q_bytes + 2 * kv_bytes);
+        for (int u = warp; u < q_units + 2 * kv_units; u += kAppendWarps) {
+            const bool is_q = u < q_units, is_k = !is_q && u < q_units + kv_units;
+            const int h = 4 * (is_q ? u : is_k ? u - q_units : u - q_units - kv_units) + (lane >> 3);
+            const bool live = h < (is_q ? a.q_heads : c.kv_heads);
+            const uint4* src = reinterpret_cast<const uint4*>(st + (is_q ? 0 : is_k ? q_bytes : q_bytes + kv_bytes) + h * 256);
+            uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
+            if (live) x = src[sub], y = src[sub + 8];
+            if (is_q || is_k) {
+                Rotation turn;
+                turn.make(is_q ? qn0 : kn0, is_q ? qn1 : kn1, cos_row, cos_row + 64, sub);
+                turn.apply(x, y, a.eps);
+            }
+            if (live) {
+                uint4* to = reinterpret_cast<uint4*>(is_q ? a.q_out + r.x * a.q_out_stride + h * kCacheHd
+                                                          : (is_k ? c.k : c.v) + cache_kv_offset(c, page, h, r.z));
+                to[sub] = x;
+                to[sub + 8] = y;
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.empty[s]);
+        if (warp == kAppendWarps - 1) {
+            append_state(c, r.y, r.z, r.w, lane);
+            if (a.lens_out && lane == 0) a.lens_out[r.x] = r.z + 1;
+        }
+        if (++s == stages) s = 0, ++round;
+    }
 }
 
 // The handle's device for the length of a call; the caller's afterwards.
@@ -130,8 +349,27 @@ int launched(cudaError_t e, const char* what) {
 
 }  // namespace
 
-cudaError_t launch_cache_append(const CacheAppendArgs& a, cudaStream_t s) {
-    return launch_after(cache_append_kernel, dim3(a.n), kAppendWarps * 32, 0, s, a);
+cudaError_t launch_cache_append(const CacheAppendArgs& a, int sms, cudaStream_t s) {
+    const int q_units = (a.q_heads + 3) / 4, kv_units = (a.c.kv_heads + 3) / 4;
+    const int stage = (a.q_heads + 2 * a.c.kv_heads) * kCacheHd * 2 + 512;
+    // From four rows an SM on the ring pays: 4001 rows of 64 + 8 + 8 heads take 60 us a CTA a row
+    if (a.n >= 4 * sms && 2 * stage <= kAppendRing) {
+        const int stages = std::min(kAppendStages, kAppendRing / stage);
+        static std::atomic<uint64_t> configured{0};
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = 1ull << (dev & 63);
+        if (!(configured.load() & bit)) {
+            e = cudaFuncSetAttribute(cache_append_stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kAppendRing);
+            if (e != cudaSuccess) return e;
+            configured.fetch_or(bit);
+        }
+        return launch_after(cache_append_stream_kernel, dim3(sms), kAppendWarps * 32 + 32,
+                            static_cast<size_t>(stages) * stage, s, a, stages, stage);
+    }
+    const int warps = std::min(q_units + 2 * kv_units, kAppendWarps);
+    return launch_after(cache_append_kernel, dim3(a.n), warps * 32, 0, s, a);
 }
 
 }  // namespace q3
@@ -220,7 +458,7 @@ int q3_cache_append(q3_cache* c, const uint16_t* q, size_t q_stride, const uint1
              "q3_cache_append: null pointer");
     if (n == 0) return Q3_OK;
     const CacheView& w = c->view;
-    Q3_CHECK(n <= INT_MAX, "q3_cache_append: too many rows");
+    Q3_CHECK(n <= (1u << 24), "q3_cache_append: too many rows");
     Q3_CHECK(row_seq || n <= static_cast<size_t>(w.rows), "q3_cache_append: more rows than sequences");
     Q3_CHECK(q_heads >= 1 && q_heads <= 65536, "q3_cache_append: q_heads must be 1 .. 65536");
     Q3_CHECK(max_pos >= 1 && max_pos <= INT_MAX, "q3_cache_append: max_pos");
@@ -231,7 +469,8 @@ int q3_cache_append(q3_cache* c, const uint16_t* q, size_t q_stride, const uint1
              "q3_cache_append: row strides must be multiples of 8");
     Q3_CHECK(q_stride <= INT_MAX && k_stride <= INT_MAX && v_stride <= INT_MAX && q_out_stride <= INT_MAX,
              "q3_cache_append: row stride too large");
-    Q3_CHECK(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(q_out, 16),
+    Q3_CHECK(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(q_out, 16) && aligned(q_norm, 16) &&
+                 aligned(k_norm, 16) && aligned(cos_t, 16) && aligned(sin_t, 16),
              "q3_cache_append: 16-byte alignment required");
     DeviceScope scope(c->device);
     Q3_CUDA(scope.status);
@@ -257,7 +496,7 @@ int q3_cache_append(q3_cache* c, const uint16_t* q, size_t q_stride, const uint1
     a.q_out_stride = static_cast<long long>(q_out_stride);
     a.lens_out = lens_out;
     a.eps = eps;
-    return launched(launch_cache_append(a, static_cast<cudaStream_t>(stream)), "q3_cache_append");
+    return launched(launch_cache_append(a, c->sms, static_cast<cudaStream_t>(stream)), "q3_cache_append");
 }
 
 size_t q3_cache_attention_workspace_bytes(const q3_cache* c, size_t q_heads, int accumulate) {

@@ -65,7 +65,7 @@ struct CacheAppendArgs {
     int32_t* lens_out;
     float eps;
 };
-cudaError_t launch_cache_append(const CacheAppendArgs& a, cudaStream_t s);
+cudaError_t launch_cache_append(const CacheAppendArgs& a, int sms, cudaStream_t s);
 
 struct CacheAttnArgs {
     CacheView c;

@@ -262,6 +262,59 @@ def test_append_of_a_prompt(be):
     check_append(be, s, 4, [order[r].pop() for r in seqs], rng.integers(0, 600, 477).tolist(), row_seq=seqs)
 
 
+@pytest.mark.parametrize("qh,kvh", [(64, 8), (6, 3), (1, 1), (400, 2)])
+def test_append_of_many_rows(be, qh, kvh):
+    """Enough rows for the streaming form (and, with 400 query heads, rows too long for it): rows left out, rows with bad
+    values among them, every other row as in the plain form."""
+    import torch
+
+    from inference_b200 import Q3Error
+
+    n = 1300
+    s = Setup(3, kvh, 700, seed=qh)
+    rng = np.random.default_rng(qh)
+    order = {r: rng.permutation(700).tolist() for r in range(3)}
+    seqs = [int(x) for x in rng.integers(0, 3, n)]
+    slots = [order[r].pop() for r in seqs]
+    token_pos = [int(x) for x in rng.integers(0, 600, n)]
+    left_out = sorted(set(int(x) for x in rng.integers(0, n, 60)))
+    for j, i in enumerate(left_out):
+        if j % 3 == 0:
+            slots[i] = -1
+        elif j % 3 == 1:
+            token_pos[i] = 600 + j
+        else:
+            slots[i] = 700 + j
+    live = torch.ones(n, dtype=torch.bool, device="cuda")
+    live[ints(left_out).long()] = False
+    rope = tables(be)
+    wide = s.randn(n, qh + 2 * kvh, HD)
+    q, k, v = wide.split([qh, kvh, kvh], dim=1)
+    qn, kn = s.randn(HD), s.randn(HD)
+    pos = ints(token_pos).long().clamp(0, 599)
+    want_k, want_v, want_w, want_p = s.k.clone(), s.v.clone(), s.w.clone(), s.pos.clone()
+    q_out = torch.full((n, qh, HD), 5.0, dtype=torch.bfloat16, device="cuda")
+    lens_out = torch.full((n,), 99, dtype=torch.int32, device="cuda")
+    with s.cache() as cache:
+        be.cache_append(cache, q, k, v, qn, kn, rope, ints(token_pos), ints(slots), q_out, EPS, lens_out=lens_out,
+                        row_seq=ints(seqs))
+        with pytest.raises(Q3Error):
+            cache.sync()
+    zq, tq = cu.turn(q, qn, rope.cosine[pos], rope.sine[pos], EPS)
+    close(q_out[live], zq[live], tq[live], "query")
+    assert (q_out[~live] == 5.0).all() and (lens_out[~live] == 99).all()
+    slot, seq = ints(slots).long()[live], ints(seqs).long()[live]
+    assert torch.equal(lens_out[live].long(), slot + 1)
+    page, at = s.tables[seq, slot // PAGE].long(), slot % PAGE
+    zk, tk = cu.turn(k, kn, rope.cosine[pos], rope.sine[pos], EPS)
+    close(s.k[page, :, at], zk[live], tk[live], "key")
+    want_k[page, :, at] = s.k[page, :, at]
+    want_v[page, :, at] = v[live]
+    want_w[seq, :, slot] = 0.0
+    want_p[seq, :, slot] = ints(token_pos)[live][:, None]
+    assert same(s.k, want_k) and same(s.v, want_v) and same(s.w, want_w) and same(s.pos, want_p)
+
+
 @pytest.mark.parametrize("what,row", [("slot", (200, 5, 0)), ("slot", (-2, 5, 0)), ("position", (3, 600, 0)),
                                       ("position", (3, -1, 0)), ("sequence", (3, 5, 2)), ("sequence", (3, 5, -1)),
                                       ("page", (70, 5, 1))])
