@@ -276,6 +276,9 @@ __global__ void __launch_bounds__(kAppendWarps * 32 + 32, 1)
     const uint4 qn0 = reinterpret_cast<const uint4*>(a.q_norm)[sub], qn1 = reinterpret_cast<const uint4*>(a.q_norm)[sub + 8];
     const uint4 kn0 = reinterpret_cast<const uint4*>(a.k_norm)[sub], kn1 = reinterpret_cast<const uint4*>(a.k_norm)[sub + 8];
     const int q_units = (a.q_heads + 3) / 4, kv_units = (c.kv_heads + 3) / 4;
+    // the rows' units one after the other, dealt to the warps: a warp's first unit of the row at hand
+    const int units = q_units + 2 * kv_units, shift = units % kAppendWarps;
+    int first = warp;
     for (int s = 0, round = 0;;) {
         if (!mbar_wait(&sm.full[s], round & 1, c.err, DEV_TMA_WAIT_TIMEOUT)) return;
         const int4 r = sm.row[s];
@@ -283,7 +286,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32 + 32, 1)
         const int page = sm.page[s];
         const uint8_t* st = ring + static_cast<size_t>(s) * stage_bytes;
         const float* cos_row = reinterpret_cast<const float*>(st + q_bytes + 2 * kv_bytes);
-        for (int u = warp; u < q_units + 2 * kv_units; u += kAppendWarps) {
+        for (int u = first; u < units; u += kAppendWarps) {
             const bool is_q = u < q_units, is_k = !is_q && u < q_units + kv_units;
             const int h = 4 * (is_q ? u : is_k ? u - q_units : u - q_units - kv_units) + (lane >> 3);
             const bool live = h < (is_q ? a.q_heads : c.kv_heads);
@@ -309,6 +312,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32 + 32, 1)
             if (a.lens_out && lane == 0) a.lens_out[r.x] = r.z + 1;
         }
         if (++s == stages) s = 0, ++round;
+        first = first < shift ? first + kAppendWarps - shift : first - shift;
     }
 }
 
