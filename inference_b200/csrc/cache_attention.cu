@@ -159,7 +159,8 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
 
     if (warp == kWarps) {
         // ------------------------------------------------------------ producer
-        const Plan plan = plan_make(sm.before[kThreads] * c.kv_heads, parts.workers);
+        const int total = sm.before[kThreads] * c.kv_heads;
+        const Plan plan = plan_make(total, parts.workers);
         const uint64_t pol = policy_evict_first();
         int k = 0;        // tiles issued
         bool ok = true;
@@ -175,21 +176,26 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
             if (lane == 0 && plan.chunks > gridDim.x) next = gridDim.x + static_cast<int>(atomicAdd(c.next_chunk, 1u));
             int t0, t1, place;
             plan_chunk(plan, chunk, t0, t1, place);
-            for (int i0 = t0; i0 < t1 && ok; i0 += 32) {
+            // the chunk's cuts may have moved by up to kPlanReach tiles
+            const int stop = min(total, t1 + kPlanReach);
+            for (int i0 = max(0, t0 - kPlanReach); i0 < stop && ok; i0 += 32) {
                 // lane i: tile i0 + i
                 int4 d = make_int4(0, 0, 0, 0);
                 int y = 0;
-                if (i0 + lane < t1) {
+                bool here = false;
+                if (i0 + lane < stop) {
                     const int t = i0 + lane;
                     const PlanPlace p = locate<kThreads>(t, a.lens, c, sm.before);
-                    const int page = c.tables[p.row * c.table_stride + p.tile];
                     const int run0 = t - p.tile;
-                    const bool begins = run0 >= t0, ends = run0 + p.tiles <= t1;
+                    auto behind = [&](int tile, int cut) { return plan_behind(run0, p.tiles, tile, cut); };
+                    here = behind(p.tile, t0) && (t1 == total || !behind(p.tile, t1));
+                    const bool begins = behind(0, t0), ends = t1 == total || !behind(p.tiles - 1, t1);
                     int flags = 0;
-                    if (p.tile == 0 || t == t0) flags |= TILE_FIRST;
-                    if (p.tile == p.tiles - 1 || t == t1 - 1) flags |= TILE_LAST;
+                    if (p.tile == 0 || !behind(p.tile - 1, t0)) flags |= TILE_FIRST;
+                    if (p.tile == p.tiles - 1 || (t1 < total && behind(p.tile + 1, t1))) flags |= TILE_LAST;
                     if (begins && ends) flags |= TILE_WHOLE;
                     if (begins) flags |= TILE_BEGIN;
+                    const int page = here ? c.tables[p.row * c.table_stride + p.tile] : 0;
                     if (page < 0 || page >= c.num_pages) {
                         flags |= TILE_BAD;
                         record_error(c.err, DEV_BAD_PAGE);
@@ -198,7 +204,8 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                     }
                     d = make_int4(p.row, p.head, t, flags | min(kCachePage, p.len - p.tile * kCachePage) << 8 | place << 16);
                 }
-                for (int i = 0; i < 32 && i0 + i < t1 && ok; ++i, ++k) {
+                for (unsigned left = __ballot_sync(0xffffffffu, here); left && ok; left &= left - 1, ++k) {
+                    const int i = __ffs(left) - 1;
                     const int4 t = make_int4(__shfl_sync(0xffffffffu, d.x, i), __shfl_sync(0xffffffffu, d.y, i),
                                              __shfl_sync(0xffffffffu, d.z, i), __shfl_sync(0xffffffffu, d.w, i));
                     const int row0 = __shfl_sync(0xffffffffu, y, i);
@@ -554,7 +561,8 @@ __global__ void __maxnreg__(64)
             const int at = __popc(sm.starts[warp] & ((1u << lane) - 1)) + (warp ? __popc(sm.starts[0]) : 0);
             const int run0 = t + tid - p.tile, here = min(n - tid, p.tiles - p.tile);
             sm.where[at] = make_int4(p.row, p.head, p.tile, min(here * kCachePage, p.len - p.tile * kCachePage));
-            const int c0 = plan_place_of(plan, run0), c1 = plan_place_of(plan, run0 + p.tiles - 1);
+            int c0, c1;
+            plan_run(plan, run0, p.tiles, c0, c1);
             int slice = 0;  // of the run's outputs, in units of 4 dims
             if (c0 != c1 && max(run0, t0) == t + tid) {  // cut, and not met before in this share
                 const int first = equal_share_of(mine, run0);

@@ -21,7 +21,10 @@
 namespace q3 {
 
 constexpr int kPlanTile = 64;
-constexpr int kPlanSmall = 3;  // no chunk but a region's last is smaller than this many tiles
+constexpr int kPlanTiered = 32;  // tiles a worker from which on work is taken dynamically
+constexpr int kPlanSmall = 4;    // the least tiles of a tier
+constexpr int kPlanSnap = 8;     // runs up to so many tiles are not cut
+constexpr int kPlanReach = 4;    // how far a cut moves to spare a run
 
 // n / d for 0 <= n < 2^31, d > 0: on the device by way of a float quotient and its
 // correction, a third of the latency of the general division.
@@ -60,12 +63,16 @@ Q3_HD int equal_share_of(const Equal& e, int t) {
 }
 
 // Every worker (CTA) has an equal region of the tiles.  Its first 5/8 are one chunk,
-// which it begins with; the rest is cut into chunks that halve down to 3 tiles and
+// which it begins with; the rest is cut into chunks that halve down to 4 tiles and
 // are taken by whichever worker is free, the larger ones of all regions first: SMs
 // differ in the bandwidth they get (on a B200, whole regions of 125 tiles took 157 to
-// 204 us), and what a worker finishes late is at most a small chunk.  Regions below 8
-// tiles stay whole.  Chunk id = tier * workers + region gives the order of taking;
-// the order along the tiles is region * tiers + tier.
+// 204 us), and what a worker finishes late is at most a small chunk.  Regions below
+// 32 tiles stay whole: more cuts cost more than they gain.  Chunk id = tier * workers +
+// region gives the order of taking; the order along the tiles is region * tiers + tier.
+//
+// A cut inside a run costs a part to write and to join, so cuts move to a run's
+// nearer end where the run has at most 8 tiles, or the end is at most 2 tiles away
+// (plan_down, plan_up).  A chunk may be empty then; those of one run are consecutive.
 Q3_HD int plan_rest(int base) { return base / 8 * 3 + base % 8 * 3 / 8; }
 struct Plan {
     Equal region;
@@ -76,7 +83,7 @@ Q3_HD Plan plan_make(int total, int workers) {
     p.region = equal_make(total, workers);
     p.workers = workers;
     p.tiers = 1;
-    if (p.region.base >= 8)
+    if (p.region.base >= kPlanTiered)
         for (int left = plan_rest(p.region.base); left >= kPlanSmall; left /= 2) ++p.tiers;
     p.chunks = p.region.base > 0 ? p.tiers * workers : p.region.extra;
     return p;
@@ -95,12 +102,29 @@ Q3_HD void plan_chunk(const Plan& p, int id, int& first, int& end, int& place) {
     end = tier + 1 < p.tiers ? begin + plan_tier(p, tier + 1) : equal_first(p.region, region + 1);
     place = region * p.tiers + tier;
 }
-// The place of the chunk that holds tile t.
+// The place of the chunk that would hold tile t if no cut moved.
 Q3_HD int plan_place_of(const Plan& p, int t) {
     const int region = equal_share_of(p.region, t), at = t - equal_first(p.region, region);
     int tier = 0;
     while (tier + 1 < p.tiers && plan_tier(p, tier + 1) <= at) ++tier;
     return region * p.tiers + tier;
+}
+// Cuts at most this many tiles behind a run's begin move to it, and cuts at most this
+// many tiles before its end to the end.
+Q3_HD int plan_down(int tiles) { return tiles <= kPlanSnap ? (tiles - 1) / 2 : 2; }
+Q3_HD int plan_up(int tiles) { return tiles <= kPlanSnap ? tiles / 2 : 2; }
+// Whether tile run0 + tile of the run [run0, run0 + tiles) lies at or behind a cut that
+// the plan has at tile `cut`, wherever that moved.
+Q3_HD bool plan_behind(int run0, int tiles, int tile, int cut) {
+    if (cut <= run0 + plan_down(tiles)) return true;
+    if (cut >= run0 + tiles - plan_up(tiles)) return false;
+    return run0 + tile >= cut;
+}
+// The places of the chunks that hold a run's first and last tile: the run's parts are
+// in the chunks at these places and between.
+Q3_HD void plan_run(const Plan& p, int run0, int tiles, int& first, int& last) {
+    first = plan_place_of(p, run0 + plan_down(tiles));
+    last = plan_place_of(p, run0 + tiles - plan_up(tiles) - 1);
 }
 
 // Rows are scanned in `groups` groups of consecutive rows; before[i] = tiles of one

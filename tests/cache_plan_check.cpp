@@ -1,5 +1,6 @@
 // Checks the work shares of the attention over a bounded paged cache
 // (csrc/cache_plan.hpp) against a brute-force walk; run by test_cache.py.
+#include <algorithm>
 #include <climits>
 #include <cstdio>
 #include <cstdlib>
@@ -32,7 +33,7 @@ static void check_totals(int total, int workers) {
         REQUIRE(at[place].first < 0);
         at[place] = {first, end};
         REQUIRE(plan_place_of(p, first) == place && plan_place_of(p, end - 1) == place);
-        REQUIRE(p.region.base < 8 || end - first >= kPlanSmall);
+        REQUIRE(p.region.base < kPlanTiered || end - first >= kPlanSmall);
     }
     int next = 0;
     for (const auto& c : at)
@@ -76,27 +77,44 @@ static void check(const std::vector<int32_t>& lens, int kvh, int max_len, int wo
         for (int r = i * per; r < rows && r < (i + 1) * per; ++r) before[i + 1] += plan_tiles(lens[r], max_len);
     }
     REQUIRE(before[groups] * kvh == total);
+    // every tile in exactly one chunk, found within reach of the unmoved chunk; a run's tiles in the chunks at
+    // its places, each with a tile of it at least; a short run in one chunk
+    std::vector<int> owner(total, -1);
     std::set<std::pair<int, int>> used;
+    int next = 0;  // chunks in order of their places hold the tiles in order
+    std::vector<std::pair<int, int>> order;
     for (int c = 0; c < plan.chunks; ++c) {
         int t0 = 0, t1 = 0, place = 0;
         plan_chunk(plan, c, t0, t1, place);
-        for (int t = t0; t < t1; ++t) {
+        order.push_back({place, c});
+    }
+    std::sort(order.begin(), order.end());
+    for (const auto& o : order) {
+        int t0 = 0, t1 = 0, place = 0;
+        plan_chunk(plan, o.second, t0, t1, place);
+        for (int t = t0 - kPlanReach < 0 ? 0 : t0 - kPlanReach; t < total && t < t1 + kPlanReach; ++t) {
             const PlanPlace p = plan_locate(t, lens.data(), rows, max_len, kvh, before.data(), groups);
             const T& w = all[t];
             REQUIRE(p.row == w.row && p.head == w.head && p.tile == w.tile && p.tiles == w.tiles &&
                     p.len == lens[w.row]);
-            const bool first = t == t0 || w.tile == 0;
-            const bool whole = w.run0 >= t0 && w.run0 + w.tiles <= t1;
-            const int c0 = plan_place_of(plan, w.run0), c1 = plan_place_of(plan, w.run0 + w.tiles - 1);
-            REQUIRE((c0 == c1) == whole);
-            if (first && !whole) {  // a part: its slot is its own, and follows from the run's first chunk
-                const int slot = w.run0 >= t0 ? 1 : 0;
-                REQUIRE(used.insert({place, slot}).second);
-                REQUIRE(c0 <= place && place <= c1);
-                REQUIRE((place == c0) == (slot == 1));
+            const bool here = plan_behind(w.run0, w.tiles, w.tile, t0) && (t1 == total || !plan_behind(w.run0, w.tiles, w.tile, t1));
+            if (!here) continue;
+            REQUIRE(owner[t] < 0 && t == next);
+            owner[t] = place;
+            ++next;
+            int c0 = 0, c1 = 0;
+            plan_run(plan, w.run0, w.tiles, c0, c1);
+            REQUIRE(c0 <= place && place <= c1);
+            if (w.tile == 0) REQUIRE(place == c0);
+            if (w.tile == w.tiles - 1) REQUIRE(place == c1);
+            if (w.tiles <= kPlanSnap) REQUIRE(c0 == c1);
+            if (c0 != c1 && (w.tile == 0 || owner[t - 1] != place)) {  // a part: its slot is its own
+                REQUIRE(place == c0 || owner[t - 1] == place - 1);
+                REQUIRE(used.insert({place, place == c0 ? 1 : 0}).second);
             }
         }
     }
+    REQUIRE(next == total);
 }
 
 int main() {
@@ -111,6 +129,7 @@ int main() {
         }
         check(lens, pick(1, 9), max_len, pick(1, 300), pick(0, 1) ? 160 : 512);
     }
+    check({20000, 3, 500, 9000, 512, 513, 20000}, 3, 20000, 20, 160);
     check(std::vector<int32_t>(4096, 1), 1, 1, 296, 160);
     check(std::vector<int32_t>(4096, 65), 2, 130, 296, 512);
     check({1000000}, 3, 1 << 20, 296, 160);
