@@ -79,6 +79,13 @@ struct Parts {
     int workers, heads;
 };
 
+// 2^x by the exponential unit: off by 2 units of 2^-23 at most, results below 2^-126 are 0.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Groups of consecutive rows, one per thread: before[t] = tiles (of one kv head)
 // before thread t's rows, before[threads] = all.
 template <int THREADS>
@@ -171,9 +178,6 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
         };
         int chunk = blockIdx.x;
         while (ok && chunk < plan.chunks) {
-            // the chunk after this one, asked for ahead: whoever is free first takes the next
-            int next = plan.chunks;
-            if (lane == 0 && plan.chunks > gridDim.x) next = gridDim.x + static_cast<int>(atomicAdd(c.next_chunk, 1u));
             int t0, t1, place;
             plan_chunk(plan, chunk, t0, t1, place);
             // the chunk's cuts may have moved by up to kPlanReach tiles
@@ -244,6 +248,9 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                     if (!ok) --k;
                 }
             }
+            // the next chunk, when this one's last copies are on their way: whoever is free first takes it
+            int next = plan.chunks;
+            if (lane == 0 && plan.chunks > gridDim.x) next = gridDim.x + static_cast<int>(atomicAdd(c.next_chunk, 1u));
             chunk = __shfl_sync(0xffffffffu, next, 0);
         }
         if (lane == 0) {
@@ -329,6 +336,7 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                 }
             }
             uint32_t ph[NT][2], pl[NT][2];
+            float score[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 // slots g (elements 0, 1) and g + 8 (2, 3), heads 2 t4 (0, 2) and 2 t4 + 1 (1, 3)
@@ -337,15 +345,6 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     sc[e] = tok + (e >> 1) * 8 < valid ? (sa[nt][e] + sb[nt][e]) * kScoreScale : -INFINITY;
-                if (a.accumulate) {
-                    float* to = parts.score + (static_cast<size_t>(d.z) * kCachePage + tok) * G + h0;
-#pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                        if (tok + 8 * r < valid) {
-                            if (h0 < G) to[8 * r * G] = sc[2 * r];
-                            if (h0 + 1 < G) to[8 * r * G + 1] = sc[2 * r + 1];
-                        }
-                }
                 float mx[2] = {fmaxf(sc[0], sc[2]), fmaxf(sc[1], sc[3])};
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) {
@@ -354,22 +353,27 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                 }
                 float p[4], corr[2];
 #pragma unroll
+                for (int e = 0; e < 4; ++e) score[nt][e] = sc[e];
+#pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const float mn = fmaxf(m_run[nt][j], mx[j]);
                     // nothing above -infinity yet: the exponentials' base is 0, not -infinity
                     const float base = mn == -INFINITY ? 0.f : mn;
-                    corr[j] = exp2f(m_run[nt][j] - base);
-                    p[j] = exp2f(sc[j] - base);
-                    p[j + 2] = exp2f(sc[j + 2] - base);
+                    corr[j] = ex2(m_run[nt][j] - base);
+                    p[j] = ex2(sc[j] - base);
+                    p[j + 2] = ex2(sc[j + 2] - base);
                     m_run[nt][j] = mn;
                     l_run[nt][j] = l_run[nt][j] * corr[j] + p[j] + p[j + 2];
                 }
+                // a new maximum (seldom after a run's first tiles) rescales what there is
+                if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
-                for (int dt = 0; dt < 8; ++dt) {
-                    o[nt][dt][0] *= corr[0];
-                    o[nt][dt][1] *= corr[1];
-                    o[nt][dt][2] *= corr[0];
-                    o[nt][dt][3] *= corr[1];
+                    for (int dt = 0; dt < 8; ++dt) {
+                        o[nt][dt][0] *= corr[0];
+                        o[nt][dt][1] *= corr[1];
+                        o[nt][dt][2] *= corr[0];
+                        o[nt][dt][3] *= corr[1];
+                    }
                 }
                 // P as two BF16 parts: the second holds what the first's rounding left
                 bf16 hi[4], lo[4];
@@ -395,6 +399,25 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                         mma_bf16_16816(o[nt][dt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
                         mma_bf16_16816(o[nt][dt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
                     }
+                }
+            }
+            if (a.accumulate) {
+                const int tok = warp * 16 + g;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const int h0 = nt * 8 + 2 * t4;
+                    float* to = parts.score + (static_cast<size_t>(d.z) * kCachePage + tok) * G + h0;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        if (tok + 8 * r < valid && h0 < G) {
+                            if (G % 2 == 0) {
+                                *reinterpret_cast<float2*>(to + 8 * r * G) =
+                                    make_float2(score[nt][2 * r], score[nt][2 * r + 1]);
+                            } else {
+                                to[8 * r * G] = score[nt][2 * r];
+                                if (h0 + 1 < G) to[8 * r * G + 1] = score[nt][2 * r + 1];
+                            }
+                        }
                 }
             }
         }
@@ -433,7 +456,7 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                 const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
-                    f[w] = exp2f(sm.m[w][h] - base);
+                    f[w] = ex2(sm.m[w][h] - base);
                     L += sm.l[w][h] * f[w];
                 }
                 const float inv = poisoned ? 0.f : 1.f / L;
@@ -521,9 +544,9 @@ __device__ __forceinline__ void add_weights(float* w, const float* s, const floa
             float p = 0.f;
             if constexpr (GV > 0) {
 #pragma unroll
-                for (int h = 0; h < GV; ++h) p += exp2f(sc[u][h] - ml[h].x) * ml[h].y;
+                for (int h = 0; h < GV; ++h) p += ex2(sc[u][h] - ml[h].x) * ml[h].y;
             } else if (j < n) {
-                for (int h = 0; h < G; ++h) p += exp2f(s[static_cast<size_t>(j) * G + h] - ml[h].x) * ml[h].y;
+                for (int h = 0; h < G; ++h) p += ex2(s[static_cast<size_t>(j) * G + h] - ml[h].x) * ml[h].y;
             }
             if (j < n) w[j] = x[u] + p;
         }
@@ -608,13 +631,13 @@ __global__ void __maxnreg__(64)
                             m = fmaxf(m, x[u].x);
                         }
                         const float base = m == -INFINITY ? 0.f : m;
-                        l *= exp2f(before - base);
+                        l *= ex2(before - base);
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) l += x[u].y * exp2f(x[u].x - base);
+                        for (int u = 0; u < 8; ++u) l += x[u].y * ex2(x[u].x - base);
                     }
                 float M = m;
                 for (int off = wide; off < 32; off <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-                l *= exp2f(m - (M == -INFINITY ? 0.f : M));
+                l *= ex2(m - (M == -INFINITY ? 0.f : M));
                 for (int off = wide; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
                 bad = __any_sync(0xffffffffu, bad);
                 if (lane < wide) sm.part[r][warp][lane] = make_float2(bad ? INFINITY : M, bad ? 0.f : l);
@@ -639,7 +662,7 @@ __global__ void __maxnreg__(64)
                         }
                         const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
-                        for (int i = 0; i < kJoinWarps; ++i) L += x[i].y * exp2f(x[i].x - base);
+                        for (int i = 0; i < kJoinWarps; ++i) L += x[i].y * ex2(x[i].x - base);
                         sm.ml[r][h] = make_float2(base, bad ? 0.f : 1.f / L);
                     }
                 }
@@ -659,7 +682,7 @@ __global__ void __maxnreg__(64)
 #pragma unroll 4
                         for (int s = c0 + turn; s <= c1; s += turns) {
                             const size_t at = static_cast<size_t>(s * 2 + (s == c0)) * G + h;
-                            const float f = exp2f(parts.pml[at].x - ml.x);
+                            const float f = ex2(parts.pml[at].x - ml.x);
                             const float4 v = reinterpret_cast<const float4*>(parts.po + at * kCacheHd)[unit % (kCacheHd / 4)];
                             x.x += v.x * f, x.y += v.y * f, x.z += v.z * f, x.w += v.w * f;
                         }

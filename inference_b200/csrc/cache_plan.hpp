@@ -22,7 +22,7 @@ namespace q3 {
 
 constexpr int kPlanTile = 64;
 constexpr int kPlanTiered = 32;  // tiles a worker from which on work is taken dynamically
-constexpr int kPlanSmall = 4;    // the least tiles of a tier
+constexpr int kPlanSmall = 3;    // the least tiles of a tier
 constexpr int kPlanSnap = 8;     // runs up to so many tiles are not cut
 constexpr int kPlanReach = 4;    // how far a cut moves to spare a run
 
@@ -63,7 +63,7 @@ Q3_HD int equal_share_of(const Equal& e, int t) {
 }
 
 // Every worker (CTA) has an equal region of the tiles.  Its first 5/8 are one chunk,
-// which it begins with; the rest is cut into chunks that halve down to 4 tiles and
+// which it begins with; the rest is cut into chunks that halve down to 3 tiles and
 // are taken by whichever worker is free, the larger ones of all regions first: SMs
 // differ in the bandwidth they get (on a B200, whole regions of 125 tiles took 157 to
 // 204 us), and what a worker finishes late is at most a small chunk.  Regions below
