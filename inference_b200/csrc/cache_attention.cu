@@ -169,12 +169,10 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
         const int total = sm.before[kThreads] * c.kv_heads;
         const Plan plan = plan_make(total, parts.workers);
         const uint64_t pol = policy_evict_first();
-        int k = 0;        // tiles issued
+        int k = 0, s = 0, round = 0;  // tiles sent for; the stage for the next, used `round` times before
         bool ok = true;
-        // a stage to fill: the k-th
         auto stage_free = [&]() {
-            if (k < S) return true;
-            return mbar_wait(&sm.empty[k % S], ((k / S) - 1) & 1, c.err, DEV_TMA_WAIT_TIMEOUT);
+            return round == 0 || mbar_wait(&sm.empty[s], (round - 1) & 1, c.err, DEV_TMA_WAIT_TIMEOUT);
         };
         int chunk = blockIdx.x;
         while (ok && chunk < plan.chunks) {
@@ -208,44 +206,45 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                     }
                     d = make_int4(p.row, p.head, t, flags | min(kCachePage, p.len - p.tile * kCachePage) << 8 | place << 16);
                 }
-                for (unsigned left = __ballot_sync(0xffffffffu, here); left && ok; left &= left - 1, ++k) {
+                // each lane sends for its own tile in turn
+                for (unsigned left = __ballot_sync(0xffffffffu, here); left && ok; left &= left - 1) {
                     const int i = __ffs(left) - 1;
-                    const int4 t = make_int4(__shfl_sync(0xffffffffu, d.x, i), __shfl_sync(0xffffffffu, d.y, i),
-                                             __shfl_sync(0xffffffffu, d.z, i), __shfl_sync(0xffffffffu, d.w, i));
-                    const int row0 = __shfl_sync(0xffffffffu, y, i);
-                    if (lane == 0) {
+                    if (lane == i) {
                         ok = stage_free();
-                        const int s = k % S;
-                        if (ok && (t.w & TILE_BAD)) {
-                            sm.tile[s] = t;
-                            mbar_arrive(&sm.full[s]);
-                        } else if (ok) {
-                            sm.tile[s] = t;
-                            uint8_t* st = sm.ring[s];
-                            const int boxes = (((t.w >> 8) & 127) + 15) / 16;  // of 16 slots
-                            const uint32_t q_bytes = (t.w & TILE_FIRST) ? G * kCacheHd * 2 : 0;
-                            mbar_arrive_expect_tx(&sm.full[s], boxes * (2 * 16 * kCacheHd * 2) + q_bytes);
-                            if (boxes == 4) {
-                                for (int h = 0; h < 2; ++h) {
-                                    tma_tile(st + h * 8192, &maps.k64, h * 64, row0, &sm.full[s], pol);
-                                    tma_tile(st + kTileBytes + h * 8192, &maps.v64, h * 64, row0, &sm.full[s], pol);
-                                }
+                        if (ok) {
+                            sm.tile[s] = d;
+                            if (d.w & TILE_BAD) {
+                                mbar_arrive(&sm.full[s]);
                             } else {
-                                for (int x = 0; x < boxes; ++x)
+                                uint8_t* st = sm.ring[s];
+                                const int boxes = (((d.w >> 8) & 127) + 15) / 16;  // of 16 slots
+                                const uint32_t q_bytes = (d.w & TILE_FIRST) ? G * kCacheHd * 2 : 0;
+                                mbar_arrive_expect_tx(&sm.full[s], boxes * (2 * 16 * kCacheHd * 2) + q_bytes);
+                                if (boxes == 4) {
                                     for (int h = 0; h < 2; ++h) {
-                                        uint8_t* to = st + h * 8192 + x * 2048;
-                                        tma_tile(to, &maps.k16, h * 64, row0 + 16 * x, &sm.full[s], pol);
-                                        tma_tile(to + kTileBytes, &maps.v16, h * 64, row0 + 16 * x, &sm.full[s], pol);
+                                        tma_tile(st + h * 8192, &maps.k64, h * 64, y, &sm.full[s], pol);
+                                        tma_tile(st + kTileBytes + h * 8192, &maps.v64, h * 64, y, &sm.full[s], pol);
                                     }
+                                } else {
+                                    for (int x = 0; x < boxes; ++x)
+                                        for (int h = 0; h < 2; ++h) {
+                                            uint8_t* to = st + h * 8192 + x * 2048;
+                                            tma_tile(to, &maps.k16, h * 64, y + 16 * x, &sm.full[s], pol);
+                                            tma_tile(to + kTileBytes, &maps.v16, h * 64, y + 16 * x, &sm.full[s], pol);
+                                        }
+                                }
+                                if (q_bytes)
+                                    bulk_g2s(st + 2 * kTileBytes,
+                                             a.q + d.x * a.q_stride + static_cast<size_t>(d.y) * G * kCacheHd, q_bytes,
+                                             &sm.full[s], pol);
                             }
-                            if (q_bytes)
-                                bulk_g2s(st + 2 * kTileBytes,
-                                         a.q + t.x * a.q_stride + static_cast<size_t>(t.y) * G * kCacheHd, q_bytes,
-                                         &sm.full[s], pol);
                         }
                     }
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
-                    if (!ok) --k;
+                    ok = __shfl_sync(0xffffffffu, ok, i);
+                    if (ok) {
+                        ++k;
+                        if (++s == S) s = 0, ++round;
+                    }
                 }
             }
             // the next chunk, when this one's last copies are on their way: whoever is free first takes it
@@ -256,8 +255,8 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
         if (lane == 0) {
             ok = ok && stage_free();
             if (ok) {
-                sm.tile[k % S].w = TILE_END;
-                mbar_arrive(&sm.full[k % S]);
+                sm.tile[s].w = TILE_END;
+                mbar_arrive(&sm.full[s]);
             } else {
                 // a wait ran out: leave no copy in flight behind
                 for (int i = max(0, k - S); i < k; ++i) mbar_wait(&sm.full[i % S], (i / S) & 1, nullptr, 0);
@@ -282,10 +281,9 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
     float o[NT][8][4];                       // O^T: dims 16 dt + g (+ 8), heads 8 nt + 2 t4 (+ 1)
     float m_run[NT][2], l_run[NT][2];        // of those heads: maximum (log2), this lane's share of the sum
     bool poisoned = false;
-    for (int k = 0;; ++k) {
-        const int s = k % S;
+    for (int s = 0, round = 0;; ++s == S ? (s = 0, ++round) : 0) {
         // all four warps go on or none: a wait that ran out in one of them ends them all
-        if (!consumers_all(mbar_wait(&sm.full[s], (k / S) & 1, c.err, DEV_TMA_WAIT_TIMEOUT))) return;
+        if (!consumers_all(mbar_wait(&sm.full[s], round & 1, c.err, DEV_TMA_WAIT_TIMEOUT))) return;
         const int4 d = sm.tile[s];
         if (d.w & TILE_END) return;
         uint8_t* kt = sm.ring[s];
@@ -340,7 +338,7 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 // slots g (elements 0, 1) and g + 8 (2, 3), heads 2 t4 (0, 2) and 2 t4 + 1 (1, 3)
-                const int tok = warp * 16 + g, h0 = nt * 8 + 2 * t4;
+                const int tok = warp * 16 + g;
                 float sc[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -448,38 +446,45 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
             consumers_all(true);
             const bool whole = (d.w & TILE_WHOLE) != 0;
             const int part = (d.w >> 16) * 2 + ((d.w & TILE_BEGIN) ? 1 : 0);
-            // 64 pairs of dims by 2 heads at a time: thread tid has pair tid % 64 of head tid / 64 + 2 i
-            for (int h = tid >> 6; h < G; h += 2) {
-                float M = -INFINITY, L = 0.f, f[kWarps];
+            // side by side: `across` threads a head, four dims each, all heads at once (16 heads: in four turns)
+            const int across = G <= 4 ? 32 : G <= 8 ? 16 : 8, h = tid / across;
+            if (h < G) {
+                float m[kWarps], f[kWarps], L = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.m[w][h]);
+                for (int w = 0; w < kWarps; ++w) m[w] = sm.m[w][h];
+                const float M = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                 const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
-                    f[w] = ex2(sm.m[w][h] - base);
+                    f[w] = ex2(m[w] - base);
                     L += sm.l[w][h] * f[w];
                 }
                 const float inv = poisoned ? 0.f : 1.f / L;
-                const int dd = (tid & 63) * 2;
-                float x = 0.f, y = 0.f;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const float2 v = *reinterpret_cast<const float2*>(&acc[(w * C::kHeads + h) * kAccPitch + dd]);
-                    x += v.x * f[w];
-                    y += v.y * f[w];
-                }
-                if (whole) {
-                    const float nan = __int_as_float(0x7FC00000);
-                    *reinterpret_cast<uint32_t*>(a.out + d.x * a.out_stride +
-                                                 (static_cast<size_t>(d.y) * G + h) * kCacheHd + dd) =
-                        poisoned ? pack_bf2(f2bf(nan), f2bf(nan)) : pack_bf2(f2bf(x * inv), f2bf(y * inv));
-                    if (dd == 0 && a.accumulate)
+                const size_t at = static_cast<size_t>(part) * G + h;
+                if (tid % across == 0) {
+                    if (whole)
                         parts.ml[static_cast<size_t>(d.x) * a.q_heads + d.y * G + h] = make_float2(base, inv);
-                } else {
-                    const size_t at = static_cast<size_t>(part) * G + h;
-                    *reinterpret_cast<float2*>(parts.po + at * kCacheHd + dd) = make_float2(x, y);
-                    // no other part has a poisoned one's pair: the sum to an infinite maximum is NaN
-                    if (dd == 0) parts.pml[at] = poisoned ? make_float2(INFINITY, 0.f) : make_float2(M, L);
+                    else
+                        // no other part has a poisoned one's pair: the sum to an infinite maximum is NaN
+                        parts.pml[at] = poisoned ? make_float2(INFINITY, 0.f) : make_float2(M, L);
+                }
+                for (int dd = tid % across * 4; dd < kCacheHd; dd += across * 4) {
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) {
+                        const float4 v = *reinterpret_cast<const float4*>(&acc[(w * C::kHeads + h) * kAccPitch + dd]);
+                        x.x += v.x * f[w], x.y += v.y * f[w], x.z += v.z * f[w], x.w += v.w * f[w];
+                    }
+                    if (whole) {
+                        const float nan = __int_as_float(0x7FC00000);
+                        uint2 u;
+                        u.x = poisoned ? pack_bf2(f2bf(nan), f2bf(nan)) : pack_bf2(f2bf(x.x * inv), f2bf(x.y * inv));
+                        u.y = poisoned ? u.x : pack_bf2(f2bf(x.z * inv), f2bf(x.w * inv));
+                        *reinterpret_cast<uint2*>(a.out + d.x * a.out_stride +
+                                                  (static_cast<size_t>(d.y) * G + h) * kCacheHd + dd) = u;
+                    } else {
+                        *reinterpret_cast<float4*>(parts.po + at * kCacheHd + dd) = x;
+                    }
                 }
             }
         }

@@ -26,16 +26,13 @@ constexpr int kPlanSmall = 3;    // the least tiles of a tier
 constexpr int kPlanSnap = 8;     // runs up to so many tiles are not cut
 constexpr int kPlanReach = 4;    // how far a cut moves to spare a run
 
-// n / d for 0 <= n < 2^31, d > 0: on the device by way of a float quotient and its
-// correction, a third of the latency of the general division.
-Q3_HD int plan_div(int n, int d) {
+// n / d for 0 <= n < 2^24, d > 0.
+Q3_HD int plan_quotient(int n, int d) {
 #ifdef __CUDA_ARCH__
-    int q = static_cast<int>(static_cast<float>(n) * __frcp_rn(static_cast<float>(d)));
-    // the float quotient may be off by a little either way, and n = q * d must not wrap
-    long long r = static_cast<long long>(n) - static_cast<long long>(q) * d;
-    while (r < 0) --q, r += d;
-    while (r >= d) ++q, r -= d;
-    return q;
+    // the float quotient is off by less than one
+    int q = static_cast<int>(__fdividef(static_cast<float>(n), static_cast<float>(d)));
+    const int r = n - q * d;
+    return q + (r >= d) - (r < 0);
 #else
     return n / d;
 #endif
@@ -52,14 +49,14 @@ struct Equal {
 };
 Q3_HD Equal equal_make(int total, int parts) {
     Equal e;
-    e.base = plan_div(total, parts);
+    e.base = total / parts;
     e.extra = total - e.base * parts;
     return e;
 }
 Q3_HD int equal_first(const Equal& e, int i) { return i * e.base + (i < e.extra ? i : e.extra); }
 Q3_HD int equal_share_of(const Equal& e, int t) {
     const int big = e.extra * (e.base + 1);
-    return t < big ? plan_div(t, e.base + 1) : e.extra + plan_div(t - big, e.base);
+    return t < big ? t / (e.base + 1) : e.extra + (t - big) / e.base;
 }
 
 // Every worker (CTA) has an equal region of the tiles.  Its first 5/8 are one chunk,
@@ -116,9 +113,7 @@ Q3_HD int plan_up(int tiles) { return tiles <= kPlanSnap ? tiles / 2 : 2; }
 // Whether tile run0 + tile of the run [run0, run0 + tiles) lies at or behind a cut that
 // the plan has at tile `cut`, wherever that moved.
 Q3_HD bool plan_behind(int run0, int tiles, int tile, int cut) {
-    if (cut <= run0 + plan_down(tiles)) return true;
-    if (cut >= run0 + tiles - plan_up(tiles)) return false;
-    return run0 + tile >= cut;
+    return (cut <= run0 + plan_down(tiles)) | ((cut < run0 + tiles - plan_up(tiles)) & (run0 + tile >= cut));
 }
 // The places of the chunks that hold a run's first and last tile: the run's parts are
 // in the chunks at these places and between.
@@ -127,7 +122,14 @@ Q3_HD void plan_run(const Plan& p, int run0, int tiles, int& first, int& last) {
     last = plan_place_of(p, run0 + tiles - plan_up(tiles) - 1);
 }
 
-// Rows are scanned in `groups` groups of consecutive rows; before[i] = tiles of one
+Q3_HD int plan_log2(int n) {
+#ifdef __CUDA_ARCH__
+    return 31 - __clz(n);
+#else
+    return 31 - __builtin_clz(n);
+#endif
+}
+// Rows are scanned in `groups` (at most 256) groups of consecutive rows; before[i] = tiles of one
 // head before group i, before[groups] = all.
 Q3_HD int plan_group_rows(int rows, int groups) { return (rows + groups - 1) / groups; }
 
@@ -137,14 +139,19 @@ struct PlanPlace {
 };
 Q3_HD PlanPlace plan_locate(int t, const int32_t* lens, int rows, int max_len, int kv_heads, const int* before,
                             int groups) {
-    const int u = plan_div(t, kv_heads);  // lies in the row that holds tile u of one head
-    int lo = 0, hi = groups;              // before[lo] <= u < before[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (before[mid] <= u)
-            lo = mid;
-        else
-            hi = mid;
+    // lies in the row that holds tile u of one head
+    const int u = (kv_heads & (kv_heads - 1)) == 0 ? t >> plan_log2(kv_heads) : t / kv_heads;
+    // the last group that begins at or before u, by steps of 32, 4 and 1 groups whose loads do not wait for
+    // one another
+    int lo = 0;
+    for (int step = 32; step >= 1; step = step == 32 ? 4 : step == 4 ? 1 : 0) {
+        int n = 0;
+#ifdef __CUDA_ARCH__
+#pragma unroll
+#endif
+        for (int j = 1; j < 8; ++j)
+            if (lo + j * step < groups) n += before[lo + j * step] <= u;
+        lo += n * step;
     }
     PlanPlace p;
     p.row = lo * plan_group_rows(rows, groups);
@@ -157,7 +164,7 @@ Q3_HD PlanPlace plan_locate(int t, const int32_t* lens, int rows, int max_len, i
         ++p.row;
     }
     const int rem = t - first * kv_heads;
-    p.head = plan_div(rem, p.tiles);
+    p.head = plan_quotient(rem, p.tiles);
     p.tile = rem - p.head * p.tiles;
     return p;
 }

@@ -127,11 +127,11 @@ int main() {
             const int kind = pick(0, 9);
             n = kind == 0 ? 0 : kind == 1 ? -pick(1, 100) : kind == 2 ? max_len + pick(1, 9) : pick(0, max_len);
         }
-        check(lens, pick(1, 9), max_len, pick(1, 300), pick(0, 1) ? 160 : 512);
+        check(lens, pick(1, 9), max_len, pick(1, 300), pick(0, 1) ? 160 : 128);
     }
     check({20000, 3, 500, 9000, 512, 513, 20000}, 3, 20000, 20, 160);
     check(std::vector<int32_t>(4096, 1), 1, 1, 296, 160);
-    check(std::vector<int32_t>(4096, 65), 2, 130, 296, 512);
+    check(std::vector<int32_t>(4096, 65), 2, 130, 296, 128);
     check({1000000}, 3, 1 << 20, 296, 160);
     check({0, -1, 500}, 3, 100, 296, 160);
     for (int t = 0; t < 3000; ++t) check_totals(t, pick(1, 400));
