@@ -518,13 +518,13 @@ struct JoinSmem {
 // Weights of n slots from their scores: w[j] += sum_h 2^(s[j][h] - m_h) / l_h.  GV: the
 // heads (0: any number, in `heads`); U slots a thread in flight.
 template <int GV, int U>
-__device__ __forceinline__ void add_weights(float* w, const float* s, const float2* ml, int n, int heads) {
+__device__ __forceinline__ void add_weights(float* w, const float* s, const float2* ml, int n, int heads, int me, int threads) {
     const int G = GV ? GV : heads;
-    for (int j0 = 0; j0 < n; j0 += kJoinThreads * U) {
+    for (int j0 = 0; j0 < n; j0 += threads * U) {
         float x[U], sc[U][GV ? GV : 1];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * kJoinThreads + static_cast<int>(threadIdx.x);
+            const int j = j0 + u * threads + me;
             x[u] = j < n ? w[j] : 0.f;
             if constexpr (GV > 0) {
 #pragma unroll
@@ -545,7 +545,7 @@ __device__ __forceinline__ void add_weights(float* w, const float* s, const floa
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * kJoinThreads + static_cast<int>(threadIdx.x);
+            const int j = j0 + u * threads + me;
             float p = 0.f;
             if constexpr (GV > 0) {
 #pragma unroll
@@ -673,13 +673,19 @@ __global__ void __maxnreg__(64)
                 }
             }
             __syncthreads();
+            // With few slots to write, two warps join outputs while the other two write weights; else all do both.
+            int slots = 0;
+            bool cut = false;
+            for (int r = 0; r < nr; ++r) slots += sm.where[r0 + r].w, cut = cut || sm.span[r0 + r].w != 0;
+            const bool apart = a.accumulate && cut && slots <= 4 * kJoinThreads;
+            const int o_warps = apart ? kJoinWarps / 2 : kJoinWarps;
             // ---- outputs of cut runs, in units of 4 dims: a warp takes units, its lanes their parts
-            for (int r = 0; r < nr; ++r) {
+            for (int r = 0; r < nr && warp < o_warps; ++r) {
                 const int4 w = sm.where[r0 + r], sp = sm.span[r0 + r];
                 const int u0 = sp.w >> 16, u1 = sp.w & 0xFFFF, c0 = sp.y, c1 = sp.z, P = c1 - c0 + 1;
                 const int turns = P <= 2 ? 2 : P <= 4 ? 4 : P <= 8 ? 8 : P <= 16 ? 16 : 32;
                 const int width = 32 / turns, turn = lane / width;
-                for (int u = u0 + warp * width; u < u1; u += kJoinWarps * width) {
+                for (int u = u0 + warp * width; u < u1; u += o_warps * width) {
                     const int unit = u + lane % width, h = min(unit, u1 - 1) / (kCacheHd / 4);
                     const float2 ml = sm.ml[r][h];
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -708,7 +714,8 @@ __global__ void __maxnreg__(64)
                 }
             }
             // ---- weights
-            if (a.accumulate)
+            const int w_first = apart ? kJoinThreads / 2 : 0, w_threads = kJoinThreads - w_first;
+            if (a.accumulate && tid >= w_first)
                 for (int r = 0; r < nr; ++r) {
                     const int4 w = sm.where[r0 + r];
                     const float2* ml = sm.ml[r];
@@ -718,12 +725,12 @@ __global__ void __maxnreg__(64)
                     float* to = c.weights + cache_slot_index(c, w.x, w.y) + w.z * kCachePage;
                     const float* s = parts.score + static_cast<size_t>(sm.span[r0 + r].x + w.z) * kCachePage * G;
                     switch (G) {
-                        case 1: add_weights<1, 8>(to, s, ml, w.w, G); break;
-                        case 2: add_weights<2, 6>(to, s, ml, w.w, G); break;
-                        case 4: add_weights<4, 4>(to, s, ml, w.w, G); break;
-                        case 8: add_weights<8, 2>(to, s, ml, w.w, G); break;
-                        case 16: add_weights<16, 1>(to, s, ml, w.w, G); break;
-                        default: add_weights<0, 2>(to, s, ml, w.w, G);
+                        case 1: add_weights<1, 8>(to, s, ml, w.w, G, tid - w_first, w_threads); break;
+                        case 2: add_weights<2, 6>(to, s, ml, w.w, G, tid - w_first, w_threads); break;
+                        case 4: add_weights<4, 4>(to, s, ml, w.w, G, tid - w_first, w_threads); break;
+                        case 8: add_weights<8, 2>(to, s, ml, w.w, G, tid - w_first, w_threads); break;
+                        case 16: add_weights<16, 1>(to, s, ml, w.w, G, tid - w_first, w_threads); break;
+                        default: add_weights<0, 2>(to, s, ml, w.w, G, tid - w_first, w_threads);
                     }
                 }
             __syncthreads();  // sm.ml and sm.part are the next runs'
