@@ -37,7 +37,6 @@ constexpr int kCandidates = 256;
 constexpr int kMaxCluster = 8;
 constexpr int kMovesHere = 64;  // at most so many moves a head: by the selecting CTAs
 constexpr int kMoveThreads = 256;
-constexpr int kMoveChunk = 64;
 static_assert(kCandidates * 2 == kThreads, "two threads rank a candidate");
 
 // Larger key = kept earlier.  Slots of the recent window come before every
@@ -79,34 +78,40 @@ struct Smem {
     uint32_t words[];         // bitmap of the piece's kept slots, then their keys
 };
 
-// Moves i = first, first + step, ... below n, each by the 16 lanes that share `first`:
-// 16 bytes of K and of V a lane, four moves in flight.
+// Moves of the lists' entries [first, first + 16) below n by 16 lanes: a lane looks up one
+// entry (and moves its weight and position), all of them move its K and V, 16 bytes each
+// a lane, four slots in flight.
 __device__ __forceinline__ void move_slots(const CacheEvictArgs& a, const int2* dst, const int2* src, size_t at, int first,
-                                           int step, int n) {
+                                           int n) {
     const CacheView& c = a.c;
     float* wo = a.weights_out ? a.weights_out : c.weights;
     int32_t* po = a.positions_out ? a.positions_out : c.positions;
     const int sub = threadIdx.x & 15;
+    const unsigned lanes = 0xFFFFu << (threadIdx.x & 16);
     const uint4 *kp = reinterpret_cast<const uint4*>(c.k) + sub, *vp = reinterpret_cast<const uint4*>(c.v) + sub;
+    const bool in = first + sub < n;
+    const int2 d = in ? dst[first + sub] : make_int2(0, 0), s = in ? src[first + sub] : make_int2(0, 0);
+    const float w = in ? c.weights[at + s.x] : 0.f;
+    const int32_t p = in ? c.positions[at + s.x] : 0;
     constexpr int U = 4;
-    for (int i = first; i < n; i += U * step) {
-        int2 d[U], s[U];
+#pragma unroll
+    for (int i = 0; i < 16; i += U) {
+        if (first + i >= n) break;
         uint4 k[U], v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i + u * step < n) d[u] = dst[i + u * step], s[u] = src[i + u * step];
+        for (int u = 0; u < U; ++u) {
+            const size_t of = static_cast<size_t>(__shfl_sync(lanes, s.y, i + u, 16)) * 16;
+            if (first + i + u < n) k[u] = kp[of], v[u] = vp[of];
+        }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i + u * step < n) k[u] = kp[static_cast<size_t>(s[u].y) * 16], v[u] = vp[static_cast<size_t>(s[u].y) * 16];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i + u * step < n) {
-                const_cast<uint4*>(kp)[static_cast<size_t>(d[u].y) * 16] = k[u];
-                const_cast<uint4*>(vp)[static_cast<size_t>(d[u].y) * 16] = v[u];
-                // one lane a move takes its weight, another its position
-                if (sub == 0) wo[at + d[u].x] = c.weights[at + s[u].x];
-                if (sub == 1) po[at + d[u].x] = c.positions[at + s[u].x];
-            }
+        for (int u = 0; u < U; ++u) {
+            const size_t to = static_cast<size_t>(__shfl_sync(lanes, d.y, i + u, 16)) * 16;
+            if (first + i + u < n) const_cast<uint4*>(kp)[to] = k[u], const_cast<uint4*>(vp)[to] = v[u];
+        }
+    }
+    if (in) {
+        wo[at + d.x] = w;
+        po[at + d.x] = p;
     }
 }
 
@@ -424,7 +429,9 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     }
     if (moves_here) {
         cluster_sync<C>();
-        move_slots(a, dst, src, at, rank * (kThreads / 16) + (tid >> 4), C * (kThreads / 16), n);
+        // few: four moves at a time to every 16 lanes of the cluster
+        for (int i = (rank * (kThreads / 16) + (tid >> 4)) * 4; i < n; i += C * kThreads / 4)
+            move_slots(a, dst, src, at, i, min(n, i + 4));
     } else {
         if (tid == 0 && rank == 0) m.count[rh] = n;
         if (C > 1) cluster_sync<C>();  // peers may still read this CTA's shared memory
@@ -432,15 +439,15 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     finish();
 }
 
-// 64 moves a CTA.
-__global__ void __launch_bounds__(kMoveThreads, 4) cache_evict_move_kernel(const CacheEvictArgs a, const Lists m, int chunks) {
-    const int rh = blockIdx.x / chunks, first = blockIdx.x % chunks * kMoveChunk;
+// `each` moves (4 or 16) to every 16 lanes.
+__global__ void __launch_bounds__(kMoveThreads, 4)
+    cache_evict_move_kernel(const CacheEvictArgs a, const Lists m, int chunks, int each) {
+    const int rh = blockIdx.x / chunks, first = (blockIdx.x % chunks * (kMoveThreads / 16) + (threadIdx.x >> 4)) * each;
     pdl_wait();
     pdl_trigger();
-    const int n = min(m.count[rh], first + kMoveChunk);
+    const int n = min(m.count[rh], first + each);
     const size_t list = static_cast<size_t>(rh) * m.cap;
-    move_slots(a, m.dst + list, m.src + list, static_cast<size_t>(rh) * a.c.slot_stride, first + (threadIdx.x >> 4),
-               kMoveThreads / 16, n);
+    if (first < n) move_slots(a, m.dst + list, m.src + list, static_cast<size_t>(rh) * a.c.slot_stride, first, n);
 }
 
 size_t pad16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
@@ -516,8 +523,11 @@ cudaError_t launch_cache_evict(const CacheEvictArgs& a, int sms, cudaStream_t s)
         default: e = launch_select<8>(a, m, moves_here, s);
     }
     if (e != cudaSuccess || moves_here) return e;
-    const int chunks = (m.cap + kMoveChunk - 1) / kMoveChunk;
-    return launch_after(cache_evict_move_kernel, dim3(static_cast<unsigned>(rh) * chunks), kMoveThreads, 0, s, a, m, chunks);
+    // 16 moves to 16 lanes where that still gives every SM its threads, else 4
+    const int each = rh * m.cap >= static_cast<size_t>(sms) * (2048 / 16) * 16 ? 16 : 4;
+    const int chunk = kMoveThreads / 16 * each, chunks = (m.cap + chunk - 1) / chunk;
+    return launch_after(cache_evict_move_kernel, dim3(static_cast<unsigned>(rh) * chunks), kMoveThreads, 0, s, a, m, chunks,
+                        each);
 }
 
 }  // namespace q3
