@@ -327,7 +327,9 @@ struct DeviceScope {
         else
             before = -1;
     }
+    // a failure is reported by the call, not left for the next one's cudaGetLastError
     ~DeviceScope() {
+        if (status != cudaSuccess) cudaGetLastError();
         if (before >= 0) cudaSetDevice(before);
     }
 };
@@ -407,11 +409,15 @@ int q3_cache_create(const q3_cache_desc* d, int device, q3_cache** out) {
     Q3_CHECK(aligned(d->page_tables_dev, 4) && aligned(d->weights_dev, 4) && aligned(d->positions_dev, 4) &&
                  aligned(d->state_dev, 4),
              "q3_cache_create: 4-byte aligned tables, weights, positions and state required");
-    Q3_CHECK(device >= 0, "q3_cache_create: bad device");
+    int devices = 0;
+    if (cudaGetDeviceCount(&devices) != cudaSuccess) devices = 0;
+    cudaGetLastError();  // without a GPU the descriptor can be checked all the same
+    Q3_CHECK(device >= 0 && (devices == 0 || device < devices), "q3_cache_create: no such device");
     auto* c = new (std::nothrow) q3_cache();
     if (!c) return fail(Q3_ERR_OOM, "q3_cache_create: host allocation failed");
     c->device = device;
     c->sms = num_sms(device);
+    if (devices == 0) cudaGetLastError();
     CacheView& v = c->view;
     v.k = reinterpret_cast<bf16*>(d->k_pages_dev);
     v.v = reinterpret_cast<bf16*>(d->v_pages_dev);
@@ -458,9 +464,9 @@ int q3_cache_append(q3_cache* c, const uint16_t* q, size_t q_stride, const uint1
                     const int32_t* slots, const int32_t* row_seq, size_t n, size_t q_heads, uint16_t* q_out,
                     size_t q_out_stride, int32_t* lens_out, float eps, void* stream) {
     Q3_CHECK(c, "q3_cache_append: null cache");
+    if (n == 0) return Q3_OK;
     Q3_CHECK(q && k && v && q_norm && k_norm && cos_t && sin_t && token_pos && slots && q_out,
              "q3_cache_append: null pointer");
-    if (n == 0) return Q3_OK;
     const CacheView& w = c->view;
     Q3_CHECK(n <= (1u << 24), "q3_cache_append: too many rows");
     Q3_CHECK(row_seq || n <= static_cast<size_t>(w.rows), "q3_cache_append: more rows than sequences");

@@ -33,7 +33,8 @@ def cache():
     (dict(weights=None), 1), (dict(positions=None), 1), (dict(head_dim=64), 3), (dict(page_size=16), 3),
     (dict(kv_heads=0), 1), (dict(rows=0), 1), (dict(rows=4097), 1), (dict(max_len=0), 1),
     (dict(max_len=(1 << 20) + 1), 1), (dict(max_len=129), 1), (dict(slot_stride=127), 1), (dict(num_pages=0), 1),
-    (dict(num_pages=1 << 25), 1), (dict(kv_heads=1 << 20), 1)])
+    (dict(num_pages=1 << 25), 1), (dict(kv_heads=1 << 20), 1),
+    (dict(rows=4096, kv_heads=1024, max_len=1 << 20, table_stride=1 << 14, slot_stride=1 << 20), 1)])
 def test_create_refuses(change, status):
     got, h = create(**change)
     assert got == status and not h.value
@@ -63,7 +64,7 @@ def append_args(h, **change):
     dict(c=None), dict(q=None), dict(k=None), dict(v=None), dict(q_norm=None), dict(k_norm=None), dict(cos=None),
     dict(sin=None), dict(token_pos=None), dict(slots=None), dict(q_out=None), dict(n=5), dict(n=1 << 32),
     dict(q_heads=0), dict(q_heads=5), dict(max_pos=0), dict(q_stride=516), dict(q_stride=504), dict(k_stride=128),
-    dict(v_stride=0), dict(q_out_stride=8), dict(q=1026), dict(v=1032), dict(q_out=2050)])
+    dict(v_stride=0), dict(q_out_stride=8), dict(k_norm=1028), dict(sin=1032), dict(q=1026), dict(v=1032), dict(q_out=2050)])
 def test_append_refuses(cache, change):
     from inference_b200 import lib
 
@@ -75,6 +76,7 @@ def test_append_of_nothing_is_nothing(cache):
     from inference_b200 import lib
 
     assert lib().q3_cache_append(*append_args(cache, n=0)) == 0
+    assert lib().q3_cache_append(*append_args(cache, n=0, q=None, slots=None)) == 0
 
 
 @pytest.mark.parametrize("change,status", [

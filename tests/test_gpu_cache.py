@@ -182,6 +182,79 @@ def test_attention_refuses_bad_device_values(be, bad):
     assert same(s.w[1], before[1])
 
 
+def test_attention_of_a_full_gpu(be):
+    """Enough tiles that chunks are taken dynamically, in several tiers, and runs are cut into many parts; twice, for the
+    same bits whoever takes what."""
+    import torch
+
+    lens = [20000, 19999, 1, 20000, 64, 17000, 20000, 8001]
+    s = Setup(8, 8, 20000, seed=9)
+    q = s.randn(8, 32, HD)
+    start = s.w.clone()
+    with s.cache() as cache:
+        first = check_attention(be, s, cache, q, lens)
+        after = s.w.clone()
+        for _ in range(2):
+            s.w.copy_(start)
+            out = torch.empty_like(q)
+            be.cache_attention(cache, q, ints(lens), out)
+            cache.sync()
+            assert same(out, first) and same(s.w, after)
+
+
+def test_one_very_long_sequence(be):
+    """One kv head of sixteen query heads over 150000 slots: every SM has a part of the one run."""
+    s = Setup(1, 1, 150000, seed=10)
+    q = s.randn(1, 16, HD)
+    with s.cache() as cache:
+        check_attention(be, s, cache, q, [149999])
+
+
+def test_far_offsets(be):
+    """Pages and slot state whose element offsets pass 32 bits, in all three operators."""
+    import torch
+
+    pool, kvh, rows, stride = 34000, 8, 3, 400_000_000  # 2.2e9 elements of K, 9.6e9 of weights
+    free = torch.cuda.mem_get_info()[0]
+    if free < 120 << 30:
+        pytest.skip("needs 100 GB of device memory")
+    s = Setup(rows, kvh, 200, seed=13)
+    small_k, small_v, small_tables = s.k, s.v, s.tables
+    s.k = torch.empty(pool, kvh, PAGE, HD, dtype=torch.bfloat16, device="cuda")
+    s.v = torch.empty_like(s.k)
+    s.tables = (pool - 1 - torch.arange(12, device="cuda").view(3, 4)).to(torch.int32)
+    s.k[s.tables.long().view(-1)] = small_k[small_tables.long().view(-1)]
+    s.v[s.tables.long().view(-1)] = small_v[small_tables.long().view(-1)]
+    w = torch.empty(rows, kvh, stride, dtype=torch.float32, device="cuda")[:, :, :200]
+    p = torch.empty(rows, kvh, stride, dtype=torch.int32, device="cuda")[:, :, :200]
+    w.copy_(s.w)
+    s.w, s.pos = w, p
+    lens = [199, 150, 1]
+    weights, positions, next_pos = fill_state(s, lens, seed=2, ties=False)
+    q = s.randn(rows, 32, HD)
+    rope = tables(be)
+    with s.cache() as cache:
+        check_attention(be, s, cache, q, lens)
+        weights = s.w.cpu().numpy()
+        _, moves = cu.evict(lens, next_pos, 100, 20, weights, positions)
+        lens_t, held = ints(lens), s.slots(s.k, 0, 7, 199).clone()
+        be.cache_evict(cache, lens_t, ints(next_pos), 100, 20, lens_t)
+        cache.sync()
+        now = s.slots(s.k, 0, 7, 100)
+        for a, b in zip(*moves[0, 7]):
+            held[a] = held[b]
+        assert torch.equal(now, held[:100]) and lens_t.tolist() == [100, 100, 1]
+        kv = s.randn(2, rows, kvh, HD)
+        out = torch.empty_like(q)
+        be.cache_append(cache, q, kv[0], kv[1], s.randn(HD), s.randn(HD), rope, ints([5, 6, 7]), lens_t, out, EPS,
+                        lens_out=lens_t)
+        cache.sync()
+        page = int(s.tables[2, 0])
+        assert same(s.v[page, :, 1], kv[1][2]) and int(s.pos[2, 7, 1]) == 7 and lens_t.tolist() == [101, 101, 2]
+    del s, w, p
+    torch.cuda.empty_cache()
+
+
 def test_attention_is_deterministic(be):
     import torch
 
@@ -406,6 +479,17 @@ def test_evict(be, lens, keep, recent, ties, in_place):
     check_evict(be, s, lens, keep, recent, w, p, next_pos, in_place)
 
 
+@pytest.mark.parametrize("rows,kvh,max_len,keep", [(20, 3, 8200, 3000), (10, 3, 8200, 8000), (80, 1, 21000, 5000),
+                                                   (1, 1, 200000, 60000), (2, 2, 9000, 8999), (200, 1, 70, 65)])
+@pytest.mark.parametrize("ties", [False, True])
+def test_evict_shapes(be, rows, kvh, max_len, keep, ties):
+    """Clusters of two and four, pieces too long for their keys to be kept, few and many moves, over most sequences short."""
+    lens = [max_len if r % 37 == 0 else (r * 977) % min(max_len, 400) for r in range(rows)]
+    s = Setup(rows, kvh, max_len, seed=rows)
+    w, p, next_pos = fill_state(s, lens, seed=rows + kvh, ties=ties)
+    check_evict(be, s, lens, keep, keep // 3, w, p, next_pos, in_place=not ties)
+
+
 def test_evict_equal_and_special_weights(be):
     """All weights equal (ties by slot), NaN last, infinities and negatives in order, denormals, every slot recent."""
     lens = [200] * 5
@@ -550,6 +634,87 @@ def test_captured_step_replays(be):
         ca.sync()
         cb.sync()
         del graphs
+
+
+def test_calls_behind_copies_in_a_graph(be):
+    """Captured behind a copy and a fill, not a kernel: the calls wait for them."""
+    import torch
+
+    lens, other = ints([5, 90, 0]), ints([90, 33, 64])
+    s = Setup(3, 2, 90, seed=42)
+    q = s.randn(3, 8, HD)
+    want, tol, _, _ = cu.attention(s, q, other.tolist())
+    out = torch.zeros_like(q)
+    side = torch.cuda.Stream()
+    with s.cache() as cache:
+        with torch.cuda.stream(side):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                lens.copy_(other)
+                be.cache_attention(cache, q, lens, out, accumulate=False)
+                lens.zero_()
+                be.cache_evict(cache, lens, lens, 10, 0, lens)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            out.zero_()
+            lens.fill_(1)
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            close(out, want, tol)
+            assert lens.tolist() == [0, 0, 0]
+        cache.sync()
+        del g
+
+
+def test_python_checks(be):
+    """What the Python layer refuses before the C ABI sees it."""
+    import torch
+
+    from inference_b200 import PagedCache
+
+    s = Setup(2, 2, 100, seed=1)
+    with pytest.raises(ValueError):
+        PagedCache(s.k, s.v.float(), s.tables, s.w, s.pos)
+    with pytest.raises(ValueError):
+        PagedCache(s.k, s.v, s.tables.long(), s.w, s.pos)
+    with pytest.raises(ValueError):
+        PagedCache(s.k, s.v, s.tables, s.w, None)
+    with pytest.raises(ValueError):
+        PagedCache(s.k, s.v, s.tables, s.w[:1], s.pos)
+    with pytest.raises(ValueError):
+        PagedCache(s.k, s.v, s.tables, s.w, s.pos, max_len=101)
+    with pytest.raises(ValueError):
+        PagedCache(s.k.transpose(0, 1), s.v.transpose(0, 1), s.tables)
+    q, lens, out = s.randn(2, 4, HD), ints([5, 5]), torch.empty(2, 4, HD, dtype=torch.bfloat16, device="cuda")
+    cache = s.cache()
+    for bad in (dict(query=q[:1]), dict(query=q.float()), dict(query=q.transpose(1, 2)), dict(lens=lens.long()),
+                dict(lens=lens[:1]), dict(lens=lens.cpu()), dict(output=out[:, :2]), dict(query=s.randn(2, 3, HD))):
+        with pytest.raises((ValueError, RuntimeError)):
+            be.cache_attention(cache, **{**dict(query=q, lens=lens, output=out), **bad})
+    with pytest.raises(ValueError):
+        be.cache_evict(cache, lens, lens, 0, 5, lens)
+    with pytest.raises(ValueError):
+        be.cache_evict(cache, lens, lens, 5, -1, lens)
+    with pytest.raises(ValueError):
+        be.cache_evict(cache, lens, lens, 5, 1, lens, weights_out=s.w[:, :, :50], positions_out=s.pos[:, :, :50])
+    rope = tables(be, 10)
+    kv = s.randn(2, 2, HD)
+    be.cache_append(cache, q[:0], kv[:0], kv[:0], s.randn(HD), s.randn(HD), rope, lens[:0], lens[:0], out[:0], EPS)
+    with pytest.raises(ValueError):
+        be.cache_append(cache, q, kv, kv, s.randn(HD)[:64], s.randn(HD), rope, lens, lens, out, EPS)
+    with pytest.raises(ValueError):
+        be.cache_append(cache, q, kv[:, :1], kv, s.randn(HD), s.randn(HD), rope, lens, lens, out, EPS)
+    cache.sync()
+    cache.close()
+    with pytest.raises(ValueError):
+        be.cache_attention(cache, q, lens, out)
+    plain = Setup(2, 2, 100, seed=1, weights=False)
+    with plain.cache() as c2:
+        with pytest.raises(RuntimeError, match="no weights"):
+            be.cache_attention(c2, q, lens, out)
+        be.cache_attention(c2, q, lens, out, accumulate=False)
+        c2.sync()
 
 
 def test_calls_on_two_streams(be):
