@@ -507,7 +507,7 @@ constexpr int kJoinTiles = 64;  // tiles whose runs are looked up at a time, a t
 constexpr int kJoinRuns = 8;    // runs joined between two barriers
 struct JoinSmem {
     int4 where[kJoinTiles];                      // of a run met: row, head, first tile here, slots here
-    int4 span[kJoinTiles];                       // its first tile of all, first and last chunk's place; units first << 16 | last
+    int4 span[kJoinTiles];                       // its first tile of all, first and last chunk's place; slice: turns << 24 | first unit << 12 | last
     float2 part[kJoinRuns][kJoinWarps][16];      // each warp's maximum and sum
     float2 ml[kJoinRuns][16];                    // maximum, 1 / sum (0: a bad page, no weights)
     int before[kJoinThreads + 1];
@@ -595,7 +595,11 @@ __global__ void __maxnreg__(64)
             if (c0 != c1 && max(run0, t0) == t + tid) {  // cut, and not met before in this share
                 const int first = equal_share_of(mine, run0);
                 const Equal part = equal_make(G * kCacheHd / 4, equal_share_of(mine, run0 + p.tiles - 1) - first + 1);
-                slice = equal_first(part, me - first) << 16 | equal_first(part, me - first + 1);
+                const int u0 = equal_first(part, me - first), u1 = equal_first(part, me - first + 1), P = c1 - c0 + 1;
+                // lanes that share a unit: each takes up to four parts, or fewer where lanes would be idle
+                int turns = 0;
+                while (turns < 5 && (4 << turns < P || (1 << turns < P && 64 >> turns >= u1 - u0))) ++turns;
+                slice = turns << 24 | u0 << 12 | u1;
             }
             sm.span[at] = make_int4(run0, c0, c1, slice);
         }
@@ -682,9 +686,8 @@ __global__ void __maxnreg__(64)
             // ---- outputs of cut runs, in units of 4 dims: a warp takes units, its lanes their parts
             for (int r = 0; r < nr && warp < o_warps; ++r) {
                 const int4 w = sm.where[r0 + r], sp = sm.span[r0 + r];
-                const int u0 = sp.w >> 16, u1 = sp.w & 0xFFFF, c0 = sp.y, c1 = sp.z, P = c1 - c0 + 1;
-                const int turns = P <= 2 ? 2 : P <= 4 ? 4 : P <= 8 ? 8 : P <= 16 ? 16 : 32;
-                const int width = 32 / turns, turn = lane / width;
+                const int u0 = sp.w >> 12 & 0xFFF, u1 = sp.w & 0xFFF, c0 = sp.y, c1 = sp.z;
+                const int turns = 1 << (sp.w >> 24), width = 32 / turns, turn = lane / width;
                 for (int u = u0 + warp * width; u < u1; u += o_warps * width) {
                     const int unit = u + lane % width, h = min(unit, u1 - 1) / (kCacheHd / 4);
                     const float2 ml = sm.ml[r][h];
