@@ -113,19 +113,6 @@ __device__ __forceinline__ PlanPlace locate(int t, const int32_t* lens, const Ca
     return plan_locate(t, lens, c.rows, c.max_len, c.kv_heads, before, THREADS);
 }
 
-// The consumer warps meet; whether all of them say yes.
-__device__ __forceinline__ bool consumers_all(bool yes) {
-    uint32_t all;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 p, %1, 0;\n\t"
-        "barrier.cta.red.and.pred q, 1, %2, p;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(all)
-        : "r"(static_cast<uint32_t>(yes)), "n"(kConsumers)
-        : "memory");
-    return all != 0;
-}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -281,9 +268,14 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
     float o[NT][8][4];                       // O^T: dims 16 dt + g (+ 8), heads 8 nt + 2 t4 (+ 1)
     float m_run[NT][2], l_run[NT][2];        // of those heads: maximum (log2), this lane's share of the sum
     bool poisoned = false;
+    // this lane's place in a tile's scores; whether it has a second head, and pairs are 8-byte aligned
+    float* const score_lane = parts.score + static_cast<size_t>(warp * 16 + g) * G + 2 * t4;
+    const size_t score_tile = static_cast<size_t>(kCachePage) * G;
+    const bool pairs = G % 2 == 0;
     for (int s = 0, round = 0;; ++s == S ? (s = 0, ++round) : 0) {
-        // all four warps go on or none: a wait that ran out in one of them ends them all
-        if (!consumers_all(mbar_wait(&sm.full[s], round & 1, c.err, DEV_TMA_WAIT_TIMEOUT))) return;
+        // All four warps go on or none: a wait that ran out in one of them ends them all, as the last tile does.
+        if (!mbar_wait(&sm.full[s], round & 1, c.err, DEV_TMA_WAIT_TIMEOUT)) sm.tile[s].w = TILE_END;
+        named_bar(1, kConsumers);
         const int4 d = sm.tile[s];
         if (d.w & TILE_END) return;
         uint8_t* kt = sm.ring[s];
@@ -400,28 +392,28 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                 }
             }
             if (a.accumulate) {
-                const int tok = warp * 16 + g;
+                float* const to = score_lane + static_cast<size_t>(d.z) * score_tile;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const int h0 = nt * 8 + 2 * t4;
-                    float* to = parts.score + (static_cast<size_t>(d.z) * kCachePage + tok) * G + h0;
+                    const bool h0 = nt * 8 + 2 * t4 < G, h1 = nt * 8 + 2 * t4 + 1 < G;
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                        if (tok + 8 * r < valid && h0 < G) {
-                            if (G % 2 == 0) {
-                                *reinterpret_cast<float2*>(to + 8 * r * G) =
-                                    make_float2(score[nt][2 * r], score[nt][2 * r + 1]);
-                            } else {
-                                to[8 * r * G] = score[nt][2 * r];
-                                if (h0 + 1 < G) to[8 * r * G + 1] = score[nt][2 * r + 1];
-                            }
+                    for (int r = 0; r < 2; ++r) {
+                        float* const at = to + 8 * r * G + nt * 8;
+                        const bool in = warp * 16 + g + 8 * r < valid;
+                        if (pairs) {
+                            if (in && h0)
+                                *reinterpret_cast<float2*>(at) = make_float2(score[nt][2 * r], score[nt][2 * r + 1]);
+                        } else {
+                            if (in && h0) at[0] = score[nt][2 * r];
+                            if (in && h1) at[1] = score[nt][2 * r + 1];
                         }
+                    }
                 }
             }
         }
         if (d.w & TILE_LAST) {
             // ---- merge the warps' states in warp order; finish the run or leave its part
-            consumers_all(true);  // the stage has been read by all
+            named_bar(1, kConsumers);  // the stage has been read by all
             float* acc = reinterpret_cast<float*>(kt);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -443,7 +435,7 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                             o[nt][dt][e];
             }
             wrote = true;
-            consumers_all(true);
+            named_bar(1, kConsumers);
             const bool whole = (d.w & TILE_WHOLE) != 0;
             const int part = (d.w >> 16) * 2 + ((d.w & TILE_BEGIN) ? 1 : 0);
             // side by side: `across` threads a head, four dims each, all heads at once (16 heads: in four turns)
