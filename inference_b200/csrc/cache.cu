@@ -127,7 +127,8 @@ __device__ __forceinline__ void append_state(const CacheView& c, int seq, int sl
 }
 
 // Few rows: one CTA a row, its units dealt to the warps, in the order queries, keys,
-// values.  Bound: latency.
+// values.  Bound: latency (look-ups, then loads, then stores: 2.7 us for one row of
+// 32 + 8 + 8 heads inside a graph, 3.5 us for 256).
 __global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const __grid_constant__ CacheAppendArgs a) {
     const CacheView& c = a.c;
     const int i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7;
@@ -176,7 +177,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const _
 // Many rows: a CTA an SM streams its rows (heads, and the position's cosines and sines)
 // through a shared-memory ring by bulk copies, so that up to 200 KB an SM are in flight
 // whatever the rows' look-ups wait for; 16 warps turn the heads and write them.  Bound:
-// HBM.
+// HBM: 4001 rows of 64 + 8 + 8 heads take 33.6 us, 75 % of the measured copy rate over
+// the bytes in and out; one kernel for both row counts spilled or took 51 to 64 us.
 struct AppendSmem {
     int4 row[kAppendStages];  // row (-1: the end), sequence, slot, position
     int page[kAppendStages];
@@ -358,8 +360,12 @@ int launched(cudaError_t e, const char* what) {
 cudaError_t launch_cache_append(const CacheAppendArgs& a, int sms, cudaStream_t s) {
     const int q_units = (a.q_heads + 3) / 4, kv_units = (a.c.kv_heads + 3) / 4;
     const int stage = (a.q_heads + 2 * a.c.kv_heads) * kCacheHd * 2 + 512;
-    // From four rows an SM on the ring pays: 4001 rows of 64 + 8 + 8 heads take 60 us a CTA a row
-    if (a.n >= 4 * sms && 2 * stage <= kAppendRing) {
+    // The ring takes 3 us more to start and per row about what a CTA a row spends on 24 heads, then runs at HBM's
+    // pace.  Ring against CTA a row, us (148 SMs), where it loses: 4096 rows of 4 + 1 + 1 heads 17.9 / 7.6,
+    // 1184 of 16 + 8 + 8 9.2 / 6.3, 592 of 32 + 8 + 8 7.2 / 5.9; even: 400 of 64 + 8 + 8 7.1 / 7.1; where it wins:
+    // 4096 of 16 + 8 + 8 21.5 / 24.0, 1184 of 64 + 8 + 8 12.8 / 20.3, 4096 of those 34 / 61.
+    const long long heads = a.q_heads + 2 * a.c.kv_heads;
+    if (a.n * (heads - 24) >= 150ll * sms && 2 * stage <= kAppendRing) {
         const int stages = std::min(kAppendStages, kAppendRing / stage);
         static std::atomic<uint64_t> configured{0};
         int dev = 0;
@@ -394,8 +400,8 @@ int q3_cache_create(const q3_cache_desc* d, int device, q3_cache** out) {
     Q3_CHECK(d->rows >= 1 && d->rows <= 4096, "q3_cache_create: rows must be 1 .. 4096");
     Q3_CHECK(d->max_len >= 1 && d->max_len <= (1u << 20), "q3_cache_create: max_len must be 1 .. 2^20");
     // tiles of 64 slots are numbered in 32 bits, all sequences' heads together
-    Q3_CHECK(d->rows * d->kv_heads * ((d->max_len + kCachePage - 1) / kCachePage) <= INT_MAX,
-             "q3_cache_create: rows * kv_heads * ceil(max_len / 64) must be below 2^31");
+    Q3_CHECK(d->rows * d->kv_heads * ((d->max_len + kCachePage - 1) / kCachePage) <= (1u << 30),
+             "q3_cache_create: rows * kv_heads * ceil(max_len / 64) must be at most 2^30");
     // rows of the pools are addressed by 32-bit tensor-map coordinates
     Q3_CHECK(d->num_pages >= 1 && d->num_pages <= INT_MAX / (kCachePage * d->kv_heads),
              "q3_cache_create: num_pages * kv_heads * 64 must be below 2^31");

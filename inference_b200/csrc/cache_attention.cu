@@ -21,6 +21,24 @@
 //   * probabilities need the run's final maximum and sum: the first kernel leaves
 //     the raw scores (fp32, 4 G bytes a slot, written once and mostly read back
 //     from L2), the second turns them into weights.
+//
+// mma.sync, not tcgen05: with G of 1 .. 16 query heads a 64-slot tile's two products
+// are 2 x 64 x 128 x 8 .. 16 multiply-adds against 32 KB to load, and S, P and O stay in
+// registers from one product to the next; ncu has the tensor pipe far from busy.
+//
+// Measured (B200, captured into a graph, weights accumulated; the share is that of
+// the bytes above at the measured copy rate of 6.55 TB/s):
+//   64 sequences x 8192 slots, 16 / 4 heads   204 us, 94 %  (the score stores are 8 us
+//                                             of it; the first kernel reads 1.24 GB for
+//                                             1.21 GB of K and V)
+//   one of 100001 slots, 32 / 8 heads          75 us, 83 %
+//   16 of up to 4096, 32 / 8 heads             36 us, 66 %  (join 8 us)
+//   200 of 1 .. 500, 4 / 1 heads               19 us, 25 %  (a worker's longest uncut run
+//                                             at 1 us a tile, start, join)
+//   one of 4095 14 us and one of 300 10 us    start, look-ups, one tile's latency, join
+// One kernel with a grid barrier in place of the second launch cost 2.3 us where the
+// programmatic launch costs 0.7; letting the last part of a run find its maximum and sum
+// (a fence and an atomic a part) took 50 us instead of 43 at 16 x 4096.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -73,10 +91,10 @@ static_assert(kWarps * Cfg<2>::kHeads * kAccPitch * 4 <= Cfg<2>::kStageBytes, "m
 
 struct Parts {
     float2* ml;    // [rows][q_heads]: maximum (log2) and 1 / sum of runs within one chunk (0: a bad page)
-    float2* pml;   // [chunks][2][heads]: maximum and sum of parts
-    float* po;     // [chunks][2][heads][128]: unnormalised outputs of parts
+    float2* pml;   // [chunk's place][2][G]: maximum and sum of parts
+    float* po;     // [chunk's place][2][G][128]: unnormalised outputs of parts
     float* score;  // [tile][64][G]: raw scores in log2 units
-    int workers, heads;
+    int workers;
 };
 
 // 2^x by the exponential unit: off by 2 units of 2^-23 at most, results below 2^-126 are 0.
@@ -492,7 +510,8 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
 // the maximum and sum from the run's parts, joins a slice of the run's outputs (as many
 // slices as CTAs that meet the run) and writes the weights of its own slots.  Two CTAs an
 // SM, small enough to be resident beside two of the first kernel: what depends on the
-// lengths alone (the share's runs) is done while that one runs.
+// lengths alone (the share's runs) is done while that one runs.  The lengths are safe to
+// read before the wait: the first kernel let this one start only behind its own.
 constexpr int kJoinThreads = 128;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr int kJoinTiles = 64;  // tiles whose runs are looked up at a time, a thread each
@@ -751,9 +770,10 @@ size_t max_tiles(const CacheView& c) {
     return static_cast<size_t>(c.rows) * c.kv_heads * ((c.max_len + kCachePage - 1) / kCachePage);
 }
 
-// Two resident CTAs an SM, no more than there can be tiles.
+// Two resident CTAs an SM, no more than there can be tiles, nor than 15 bits number the
+// chunks of (a region has at most 20: there are at most 2^30 tiles).
 int workers_of(const CacheView& c, int sms) {
-    return static_cast<int>(std::min(static_cast<size_t>(2 * sms), max_tiles(c)));
+    return static_cast<int>(std::min(static_cast<size_t>(std::min(2 * sms, 1024)), max_tiles(c)));
 }
 
 // The workspace's arrays from its start; returns its size.
@@ -767,7 +787,6 @@ size_t layout(const CacheView& c, int q_heads, int accumulate, int sms, uint8_t*
         return to;
     };
     p->workers = workers;
-    p->heads = G;
     p->ml = reinterpret_cast<float2*>(take(static_cast<size_t>(c.rows) * q_heads * 8));
     p->pml = reinterpret_cast<float2*>(take(parts * G * 8));
     p->po = reinterpret_cast<float*>(take(parts * G * kCacheHd * 4));
@@ -815,7 +834,8 @@ cudaError_t launch_cache_attention(const CacheAttnArgs& a, const CacheMaps& maps
     cudaError_t e = a.q_heads / c.kv_heads <= 8 ? launch_nt<1>(a, maps, parts, s) : launch_nt<2>(a, maps, parts, s);
     if (e != cudaSuccess) return e;
     // two CTAs an SM are resident beside the first kernel's; with 8 tiles a worker or more the work is worth
-    // eight, though the others start (and look up their runs) only when that one ends
+    // eight, though the others start (and look up their runs) only when that one ends: 64 x 8192 takes 220,
+    // 209, 206, 204 and 210 us with 1, 2, 3, 4 and 6 times the workers, 16 x 4096 37.1, 36.7, 36.4, 36.1 and 40.4
     const int join_ctas = max_tiles(c) >= 8 * static_cast<size_t>(parts.workers) ? 4 * parts.workers : parts.workers;
     return launch_after(cache_join_kernel, dim3(join_ctas), kJoinThreads, 0, s, a, parts);
 }

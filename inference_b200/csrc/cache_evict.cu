@@ -20,6 +20,16 @@
 // a second launch over all SMs.  Bound: latency (a dozen dependent steps of 0.3 to
 // 0.7 us) for a few evicted slots, HBM for many: 8 bytes a slot read, 1 KB a moved
 // slot.
+//
+// Measured (B200, captured into a graph), 8 kv heads:
+//   16 sequences, 2112 -> 2048 slots   9.4 us, all latency: launch, two passes of the
+//                                      select, lists, moves by the same CTAs (a second
+//                                      launch instead: 11.2 us)
+//   one, 32768 -> 4096                 22.6 us: select 13 (clusters of 8, exchanges of
+//                                      histograms), moves 9
+//   32, up to 8000 -> 2000             64 us: select 20, moves 41 at 5.75 TB/s, 88 % of
+//                                      the measured copy rate
+// Clusters of 16 CTAs and digits of 11 bits in clusters were slower.
 #include <algorithm>
 #include <atomic>
 #include <climits>

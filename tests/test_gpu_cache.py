@@ -335,10 +335,10 @@ def test_append_of_a_prompt(be):
     check_append(be, s, 4, [order[r].pop() for r in seqs], rng.integers(0, 600, 477).tolist(), row_seq=seqs)
 
 
-@pytest.mark.parametrize("qh,kvh", [(64, 8), (6, 3), (1, 1), (400, 2)])
+@pytest.mark.parametrize("qh,kvh", [(64, 8), (42, 7), (45, 1), (6, 3), (1, 1), (400, 2)])
 def test_append_of_many_rows(be, qh, kvh):
-    """Enough rows for the streaming form (and, with 400 query heads, rows too long for it): rows left out, rows with bad
-    values among them, every other row as in the plain form."""
+    """Enough rows for the streaming form (and, with few heads, rows too short for it, with 400 query heads too long): rows
+    left out, rows with bad values among them, every other row as in the plain form."""
     import torch
 
     from inference_b200 import Q3Error
