@@ -194,7 +194,7 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                     const int t = i0 + lane;
                     const PlanPlace p = locate<kThreads>(t, a.lens, c, sm.before);
                     const int run0 = t - p.tile;
-                    auto behind = [&](int tile, int cut) { return plan_behind(run0, p.tiles, tile, cut); };
+                    auto behind = [&](int tile, int cut) { return plan_behind(plan, run0, p.tiles, tile, cut); };
                     here = behind(p.tile, t0) && (t1 == total || !behind(p.tile, t1));
                     const bool begins = behind(0, t0), ends = t1 == total || !behind(p.tiles - 1, t1);
                     int flags = 0;

@@ -23,6 +23,7 @@ namespace q3 {
 constexpr int kPlanTile = 64;
 constexpr int kPlanTiered = 32;  // tiles a worker from which on work is taken dynamically
 constexpr int kPlanSmall = 3;    // the least tiles of a tier
+constexpr int kPlanWhole = 2;    // tiles a worker from which on short runs are spared
 constexpr int kPlanSnap = 8;     // runs up to so many tiles are not cut
 constexpr int kPlanReach = 4;    // how far a cut moves to spare a run
 
@@ -69,21 +70,27 @@ Q3_HD int equal_share_of(const Equal& e, int t) {
 // 73; with tiers from 12 tiles on 16 x 4096 (16 tiles) takes 37.9 us for 36.3.  Chunk id = tier * workers +
 // region gives the order of taking; the order along the tiles is region * tiers + tier.
 //
-// A cut inside a run costs a part to write and to join, so cuts move to a run's
-// nearer end where the run has at most 8 tiles, or the end is at most 2 tiles away
-// (plan_down, plan_up).  A chunk may be empty then; those of one run are consecutive.
+// A cut inside a run costs a part to write and to join, so from two tiles a worker on
+// cuts move to a run's nearer end where the run has at most 8 tiles, or the end is at
+// most 2 tiles away (plan_down, plan_up).  With less work a run's tiles side by side are
+// worth their parts: 5 tiles in each of 8 runs take 8.7 us apart and 10.3 us together,
+// 64 in each of 8 12.5 and 14.0 us; from four tiles a worker on instead of two, 200
+// sequences of 1 .. 500 slots take 19.5 us for 18.6.  A chunk may be empty then; those of one run are consecutive.
 // Sparing runs of up to 4 tiles alone, 200 sequences of 1 .. 500 slots take 19.9 us for
 // 18.7, and 20 of up to 638 with 8 heads 16.8 for 17.5.
 Q3_HD int plan_rest(int base) { return base / 8 * 3 + base % 8 * 3 / 8; }
 struct Plan {
     Equal region;
     int workers, tiers, chunks;
+    int snap, slack;  // runs up to `snap` tiles are not cut; in longer ones cuts move by up to `slack`
 };
 Q3_HD Plan plan_make(int total, int workers) {
     Plan p;
     p.region = equal_make(total, workers);
     p.workers = workers;
     p.tiers = 1;
+    p.snap = p.region.base < kPlanWhole ? 0 : kPlanSnap;
+    p.slack = p.region.base < kPlanWhole ? 0 : 2;
     if (p.region.base >= kPlanTiered)
         for (int left = plan_rest(p.region.base); left >= kPlanSmall; left /= 2) ++p.tiers;
     p.chunks = p.region.base > 0 ? p.tiers * workers : p.region.extra;
@@ -112,18 +119,18 @@ Q3_HD int plan_place_of(const Plan& p, int t) {
 }
 // Cuts at most this many tiles behind a run's begin move to it, and cuts at most this
 // many tiles before its end to the end.
-Q3_HD int plan_down(int tiles) { return tiles <= kPlanSnap ? (tiles - 1) / 2 : 2; }
-Q3_HD int plan_up(int tiles) { return tiles <= kPlanSnap ? tiles / 2 : 2; }
+Q3_HD int plan_down(const Plan& p, int tiles) { return tiles <= p.snap ? (tiles - 1) / 2 : p.slack; }
+Q3_HD int plan_up(const Plan& p, int tiles) { return tiles <= p.snap ? tiles / 2 : p.slack; }
 // Whether tile run0 + tile of the run [run0, run0 + tiles) lies at or behind a cut that
 // the plan has at tile `cut`, wherever that moved.
-Q3_HD bool plan_behind(int run0, int tiles, int tile, int cut) {
-    return (cut <= run0 + plan_down(tiles)) | ((cut < run0 + tiles - plan_up(tiles)) & (run0 + tile >= cut));
+Q3_HD bool plan_behind(const Plan& p, int run0, int tiles, int tile, int cut) {
+    return (cut <= run0 + plan_down(p, tiles)) | ((cut < run0 + tiles - plan_up(p, tiles)) & (run0 + tile >= cut));
 }
 // The places of the chunks that hold a run's first and last tile: the run's parts are
 // in the chunks at these places and between.
 Q3_HD void plan_run(const Plan& p, int run0, int tiles, int& first, int& last) {
-    first = plan_place_of(p, run0 + plan_down(tiles));
-    last = plan_place_of(p, run0 + tiles - plan_up(tiles) - 1);
+    first = plan_place_of(p, run0 + plan_down(p, tiles));
+    last = plan_place_of(p, run0 + tiles - plan_up(p, tiles) - 1);
 }
 
 Q3_HD int plan_log2(int n) {

@@ -1,7 +1,6 @@
 // Checks the work shares of the attention over a bounded paged cache
 // (csrc/cache_plan.hpp) against a brute-force walk; run by test_cache.py.
 #include <algorithm>
-#include <climits>
 #include <cstdio>
 #include <cstdlib>
 #include <random>
@@ -24,7 +23,7 @@ using namespace q3;
 static void check_totals(int total, int workers) {
     const Plan p = plan_make(total, workers);
     REQUIRE(p.tiers >= 1 && p.tiers <= 31 && p.chunks <= p.tiers * workers);
-    REQUIRE(plan_make(total < INT_MAX - 5 ? total + 5 : total, workers).tiers >= p.tiers);  // the workspace's bound
+    REQUIRE(plan_make(total + 5, workers).tiers >= p.tiers);  // the workspace's bound
     std::vector<std::pair<int, int>> at(static_cast<size_t>(p.tiers) * workers, {-1, -1});
     for (int id = 0; id < p.chunks; ++id) {
         int first = 0, end = 0, place = 0;
@@ -97,7 +96,7 @@ static void check(const std::vector<int32_t>& lens, int kvh, int max_len, int wo
             const T& w = all[t];
             REQUIRE(p.row == w.row && p.head == w.head && p.tile == w.tile && p.tiles == w.tiles &&
                     p.len == lens[w.row]);
-            const bool here = plan_behind(w.run0, w.tiles, w.tile, t0) && (t1 == total || !plan_behind(w.run0, w.tiles, w.tile, t1));
+            const bool here = plan_behind(plan, w.run0, w.tiles, w.tile, t0) && (t1 == total || !plan_behind(plan, w.run0, w.tiles, w.tile, t1));
             if (!here) continue;
             REQUIRE(owner[t] < 0 && t == next);
             owner[t] = place;
@@ -107,7 +106,7 @@ static void check(const std::vector<int32_t>& lens, int kvh, int max_len, int wo
             REQUIRE(c0 <= place && place <= c1);
             if (w.tile == 0) REQUIRE(place == c0);
             if (w.tile == w.tiles - 1) REQUIRE(place == c1);
-            if (w.tiles <= kPlanSnap) REQUIRE(c0 == c1);
+            if (w.tiles <= plan.snap) REQUIRE(c0 == c1);
             if (c0 != c1 && (w.tile == 0 || owner[t - 1] != place)) {  // a part: its slot is its own
                 REQUIRE(place == c0 || owner[t - 1] == place - 1);
                 REQUIRE(used.insert({place, place == c0 ? 1 : 0}).second);
@@ -136,7 +135,7 @@ int main() {
     check({0, -1, 500}, 3, 100, 296, 160);
     for (int t = 0; t < 3000; ++t) check_totals(t, pick(1, 400));
     for (const int workers : {1, 2, 147, 296, 1000})
-        for (const int t : {7 * workers, 8 * workers - 1, 8 * workers, 8 * workers + 1, 1000 * workers + 5, 1 << 24, INT_MAX})
+        for (const int t : {7 * workers, 8 * workers - 1, 8 * workers, 8 * workers + 1, 1000 * workers + 5, 1 << 24, 1 << 30})
             check_totals(t, workers);
     std::puts("ok");
 }

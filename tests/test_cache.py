@@ -145,6 +145,6 @@ def test_work_shares(tmp_path):
 
     src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cache_plan_check.cpp")
     exe = str(tmp_path / "cache_plan_check")
-    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=address,undefined", "-o", exe, src], check=True)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-o", exe, src], check=True)
     r = subprocess.run([exe], capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
