@@ -457,7 +457,7 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
             const bool whole = (d.w & TILE_WHOLE) != 0;
             const int part = (d.w >> 16) * 2 + ((d.w & TILE_BEGIN) ? 1 : 0);
             // side by side: `across` threads a head, four dims each, all heads at once (16 heads: in four turns)
-            const int across = G <= 4 ? 32 : G <= 8 ? 16 : 8, h = tid / across;
+            const int across_log = G <= 4 ? 5 : G <= 8 ? 4 : 3, across = 1 << across_log, h = tid >> across_log;
             if (h < G) {
                 float m[kWarps], f[kWarps], L = 0.f;
 #pragma unroll
@@ -471,14 +471,14 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                 }
                 const float inv = poisoned ? 0.f : 1.f / L;
                 const size_t at = static_cast<size_t>(part) * G + h;
-                if (tid % across == 0) {
+                if ((tid & (across - 1)) == 0) {
                     if (whole)
                         parts.ml[static_cast<size_t>(d.x) * a.q_heads + d.y * G + h] = make_float2(base, inv);
                     else
                         // no other part has a poisoned one's pair: the sum to an infinite maximum is NaN
                         parts.pml[at] = poisoned ? make_float2(INFINITY, 0.f) : make_float2(M, L);
                 }
-                for (int dd = tid % across * 4; dd < kCacheHd; dd += across * 4) {
+                for (int dd = (tid & (across - 1)) * 4; dd < kCacheHd; dd += across * 4) {
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                     for (int w = 0; w < kWarps; ++w) {
@@ -607,9 +607,9 @@ __global__ void __maxnreg__(64)
                 const int first = equal_share_of(mine, run0);
                 const Equal part = equal_make(G * kCacheHd / 4, equal_share_of(mine, run0 + p.tiles - 1) - first + 1);
                 const int u0 = equal_first(part, me - first), u1 = equal_first(part, me - first + 1), P = c1 - c0 + 1;
-                // lanes that share a unit: each takes up to four parts, or fewer where lanes would be idle
+                // lanes that share a unit: as few as take up to four parts each
                 int turns = 0;
-                while (turns < 5 && (4 << turns < P || (1 << turns < P && 64 >> turns >= u1 - u0))) ++turns;
+                while (turns < 5 && 4 << turns < P) ++turns;
                 slice = turns << 24 | u0 << 12 | u1;
             }
             sm.span[at] = make_int4(run0, c0, c1, slice);
@@ -621,8 +621,9 @@ __global__ void __maxnreg__(64)
     pdl_trigger();
     if (me == 0 && tid == 0) *c.next_chunk = 0;  // for the cache's next attention
 
-    // heads side by side in a warp: the power of two that holds G
-    const int wide = G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : G <= 8 ? 8 : 16;
+    // heads side by side in a warp: the power of two that holds G (powers of two as shifts throughout: an integer
+    // division is some 150 cycles of the chain between the two kernels)
+    const int wide_log = G <= 1 ? 0 : G <= 2 ? 1 : G <= 4 ? 2 : G <= 8 ? 3 : 4, wide = 1 << wide_log;
     for (int t = t0; t < t1; t += kJoinTiles) {
         if (t > t0) look_up(t);
         for (int r0 = 0; r0 < runs; r0 += kJoinRuns) {
@@ -631,30 +632,30 @@ __global__ void __maxnreg__(64)
             for (int r = 0; r < nr; ++r) {
                 const int c0 = sm.span[r0 + r].y, c1 = sm.span[r0 + r].z;
                 if (c0 == c1) continue;
-                const int h = tid % wide, deal = kJoinThreads / wide;
+                // (heads that there are not: the last one's, and nobody's)
+                const int h = min(tid & (wide - 1), G - 1), deal = kJoinThreads >> wide_log;
                 float m = -INFINITY, l = 0.f;
                 bool bad = false;
-                if (h < G)
-                    for (int s0 = c0 + tid / wide; s0 <= c1; s0 += 8 * deal) {
-                        float2 x[8];
+                for (int s0 = c0 + (tid >> wide_log); s0 <= c1; s0 += 8 * deal) {
+                    float2 x[8];
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            const int s = s0 + u * deal;
-                            // the run begins in chunk c0: its part there is in slot 1, the others' in slot 0
-                            x[u] = s <= c1 ? parts.pml[static_cast<size_t>(s * 2 + (s == c0)) * G + h]
-                                           : make_float2(-INFINITY, 0.f);
-                        }
-                        const float before = m;
-#pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            bad = bad || (x[u].x == INFINITY && x[u].y == 0.f);  // a bad page: see the parts
-                            m = fmaxf(m, x[u].x);
-                        }
-                        const float base = m == -INFINITY ? 0.f : m;
-                        l *= ex2(before - base);
-#pragma unroll
-                        for (int u = 0; u < 8; ++u) l += x[u].y * ex2(x[u].x - base);
+                    for (int u = 0; u < 8; ++u) {
+                        const int s = min(s0 + u * deal, c1);
+                        // the run begins in chunk c0: its part there is in slot 1, the others' in slot 0
+                        x[u] = parts.pml[static_cast<size_t>(s * 2 + (s == c0)) * G + h];
                     }
+                    const float before = m;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        if (s0 + u * deal > c1) x[u].y = 0.f, x[u].x = -INFINITY;
+                        bad |= (x[u].x == INFINITY) & (x[u].y == 0.f);  // a bad page: see the parts
+                        m = fmaxf(m, x[u].x);
+                    }
+                    const float base = m == -INFINITY ? 0.f : m;
+                    l *= ex2(before - base);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) l += x[u].y * ex2(x[u].x - base);
+                }
                 float M = m;
                 for (int off = wide; off < 32; off <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
                 l *= ex2(m - (M == -INFINITY ? 0.f : M));
@@ -677,13 +678,13 @@ __global__ void __maxnreg__(64)
 #pragma unroll
                         for (int i = 0; i < kJoinWarps; ++i) {
                             x[i] = sm.part[r][i][h];
-                            bad = bad || (x[i].x == INFINITY && x[i].y == 0.f);
+                            bad |= (x[i].x == INFINITY) & (x[i].y == 0.f);
                             M = fmaxf(M, x[i].x);
                         }
                         const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
                         for (int i = 0; i < kJoinWarps; ++i) L += x[i].y * ex2(x[i].x - base);
-                        sm.ml[r][h] = make_float2(base, bad ? 0.f : 1.f / L);
+                        sm.ml[r][h] = make_float2(base, bad ? 0.f : __fdividef(1.f, L));
                     }
                 }
             }
@@ -698,19 +699,29 @@ __global__ void __maxnreg__(64)
             for (int r = 0; r < nr && warp < o_warps; ++r) {
                 const int4 w = sm.where[r0 + r], sp = sm.span[r0 + r];
                 const int u0 = sp.w >> 12 & 0xFFF, u1 = sp.w & 0xFFF, c0 = sp.y, c1 = sp.z;
-                const int turns = 1 << (sp.w >> 24), width = 32 / turns, turn = lane / width;
+                const int turns_log = sp.w >> 24, turns = 1 << turns_log, width = 32 >> turns_log;
+                const int turn = lane >> (5 - turns_log), column = lane & (width - 1);
                 for (int u = u0 + warp * width; u < u1; u += o_warps * width) {
-                    const int unit = u + lane % width, h = min(unit, u1 - 1) / (kCacheHd / 4);
+                    const int unit = u + column, h = min(unit, u1 - 1) / (kCacheHd / 4);
                     const float2 ml = sm.ml[r][h];
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (unit < u1)
-#pragma unroll 4
-                        for (int s = c0 + turn; s <= c1; s += turns) {
+                    // four parts' loads under way together; behind the last one: that one again, with factor 0
+                    for (int s0 = c0 + turn; s0 <= c1; s0 += 4 * turns) {
+                        float m[4];
+                        float4 v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int s = min(s0 + i * turns, c1);
                             const size_t at = static_cast<size_t>(s * 2 + (s == c0)) * G + h;
-                            const float f = ex2(parts.pml[at].x - ml.x);
-                            const float4 v = reinterpret_cast<const float4*>(parts.po + at * kCacheHd)[unit % (kCacheHd / 4)];
-                            x.x += v.x * f, x.y += v.y * f, x.z += v.z * f, x.w += v.w * f;
+                            m[i] = parts.pml[at].x;
+                            v[i] = reinterpret_cast<const float4*>(parts.po + at * kCacheHd)[unit % (kCacheHd / 4)];
                         }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float f = s0 + i * turns <= c1 ? ex2(m[i] - ml.x) : 0.f;
+                            x.x += v[i].x * f, x.y += v[i].y * f, x.z += v[i].z * f, x.w += v[i].w * f;
+                        }
+                    }
                     for (int off = width; off < 32; off <<= 1) {
                         x.x += __shfl_xor_sync(0xffffffffu, x.x, off);
                         x.y += __shfl_xor_sync(0xffffffffu, x.y, off);
@@ -733,9 +744,7 @@ __global__ void __maxnreg__(64)
                 for (int r = 0; r < nr; ++r) {
                     const int4 w = sm.where[r0 + r];
                     const float2* ml = sm.ml[r];
-                    bool bad = false;
-                    for (int h = 0; h < G; ++h) bad = bad || ml[h].y == 0.f;
-                    if (bad) continue;
+                    if (ml[0].y == 0.f) continue;  // a bad page: all heads' then
                     float* to = c.weights + cache_slot_index(c, w.x, w.y) + w.z * kCachePage;
                     const float* s = parts.score + static_cast<size_t>(sm.span[r0 + r].x + w.z) * kCachePage * G;
                     switch (G) {
