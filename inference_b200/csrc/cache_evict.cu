@@ -12,8 +12,9 @@
 // its slots.  The weight of the `keep`-th slot is found by a radix select over the
 // weights' 32-bit order-preserving keys: a histogram of the next 11 bits (8 in a
 // cluster, whose CTAs read each other's through distributed shared memory) of the
-// slots that share the bits so far, until at most 256 candidates are left, which are
-// ranked by counting; usually one or two passes.  More candidates than that with all
+// slots that share the bits so far -- at first of the bits that tell usual weights
+// apart -- until at most 256 candidates are left, which are ranked by counting;
+// usually one or two passes.  More candidates than that with all
 // bits equal are a tie, cut by slot.  Then a bitmap of the kept slots, the ordered
 // lists of holes and movers from its population counts, and the moves, 16 lanes a
 // slot and tensor: by the same CTAs where at most 64 slots a head can move, else by
@@ -22,12 +23,12 @@
 // slot.
 //
 // Measured (B200, captured into a graph), 8 kv heads:
-//   16 sequences, 2112 -> 2048 slots   9.4 us, all latency: launch, two passes of the
+//   16 sequences, 2112 -> 2048 slots   9.0 us, all latency: launch, two passes of the
 //                                      select, lists, moves by the same CTAs (a second
-//                                      launch instead: 11.2 us)
-//   one, 32768 -> 4096                 22.6 us: select 13 (clusters of 8, exchanges of
+//                                      launch instead: 1.8 us more)
+//   one, 32768 -> 4096                 22.2 us: select 13 (clusters of 8, exchanges of
 //                                      histograms), moves 9
-//   32, up to 8000 -> 2000             64 us: select 20, moves 41 at 5.75 TB/s, 88 % of
+//   32, up to 8000 -> 2000             62 us: select 18, moves 41 at 5.75 TB/s, 88 % of
 //                                      the measured copy rate
 // Clusters of 16 CTAs and digits of 11 bits in clusters were slower.
 #include <algorithm>
@@ -72,6 +73,12 @@ struct Digits {
     static constexpr int kBits = C == 1 ? 11 : 8;
     static constexpr int kBins = 1 << kBits;
     static constexpr int kPer = C == 1 ? 4 : 1;  // bins a thread
+    // The first pass's bins: 32 (8) an octave for weights of 2^-44 .. 2^20 (2^-20 .. 2^12),
+    // that is the keys' bits from kShift up, less kBase; the first and the last bin take what
+    // lies outside.  (By the leading bits alone, a quarter of an octave or two octaves a bin,
+    // more candidates were left to rank: 32 of up to 8000 slots took 64.3 us for 62.2.)
+    static constexpr int kShift = C == 1 ? 18 : 20;
+    static constexpr int kBase = C == 1 ? (256 + 127 - 44) << 5 : (256 + 127 - 20) << 3;
 };
 
 struct Smem {
@@ -203,18 +210,22 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     if (bad && rank == 0) record_error(c.err, bad);
 
     // Lengths are read by every CTA of a sequence, and lens_out may be the same array: the
-    // last CTA of the grid to come here, when all have read theirs, writes it (at its end).
-    bool last = false;
-    if (tid == kThreads - 1) {
-        if (head == 0 && rank == 0) m.bad[row] = stays;
-        __threadfence();
-        last = atomicAdd(c.arrived, 1u) == gridDim.x - 1;
+    // last CTA of the grid to count itself, when all have read theirs, writes it (at its
+    // end).  Counted where no barrier waits for it (here it would be 750 cycles of the next
+    // one), and the count looked at in the end.
+    if (tid == kThreads - 1 && head == 0 && rank == 0) m.bad[row] = stays;
+    uint32_t before_me = 0;
+    auto arrive = [&]() {
+        if (tid == kThreads - 1)
+            asm volatile("atom.release.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before_me) : "l"(c.arrived) : "memory");
+    };
+    if (!moves_here) arrive();
+    auto finish = [&]() {
+        const bool last = tid == kThreads - 1 && before_me == gridDim.x - 1;
         if (last) {
             __threadfence();
             *c.arrived = 0;
         }
-    }
-    auto finish = [&]() {
         if (!__syncthreads_or(last)) return;
         for (int r = tid; r < c.rows; r += kThreads) {
             const int n = a.lens[r];
@@ -222,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
         }
     };
     if (stays || !shrinks) {
+        if (moves_here) arrive();
         if (tid == 0 && rank == 0) m.count[rh] = 0;
         if (!stays && a.weights_out)
             for (int i = wa; i < wb; i += U) {
@@ -241,15 +253,22 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     uint32_t prefix = 0;  // the keys' bits above the shift
     int need = a.keep, count = len;
     bool found = false;
-    for (int pass = 0, shift = 32 - D::kBits, bits = D::kBits; !found && bits > 0; ++pass) {
+    for (int pass = 0, shift = D::kShift, bits = D::kBits; !found && bits > 0; ++pass) {
         int* hist = sm.hist[pass & 1];
         if (pass > 0) {
             for (int i = tid; i < D::kBins; i += kThreads) hist[i] = 0;
             __syncthreads();
         }
+        auto first_bin = [](uint32_t k) {
+            return min(max(static_cast<int>(k >> D::kShift) - D::kBase, 0), D::kBins - 1);
+        };
         auto tally = [&](int s, uint32_t k) {
             const uint32_t top = k >> shift;
-            if (s < len && (pass == 0 || top >> bits == prefix)) atomicAdd(&hist[top & ((1u << bits) - 1)], 1);
+            if (pass == 0) {
+                if (s < len) atomicAdd(&hist[first_bin(k)], 1);
+            } else if (s < len && top >> bits == prefix) {
+                atomicAdd(&hist[top & ((1u << bits) - 1)], 1);
+            }
         };
         if (pass > 0) {
             each_word([&](int, int s, uint32_t k) { tally(s, k); });
@@ -302,7 +321,9 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
             above += four[i];
         }
         __syncthreads();
-        prefix = (prefix << bits) | static_cast<uint32_t>(sm.digit);
+        const int digit = sm.digit;
+        prefix = pass == 0 ? static_cast<uint32_t>(D::kBase + digit) : (prefix << bits) | static_cast<uint32_t>(digit);
+        const int before = need;
         need = sm.need;
         count = sm.count;
         if (count == need) {  // the whole bin is kept
@@ -311,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
         } else if (count <= kCandidates) {
             // few candidates: the one with need - 1 larger ones (the lower slot is the larger) is the last kept
             each_word([&](int, int s, uint32_t k) {
-                if (s < len && k >> shift == prefix)
+                if (s < len && (pass == 0 ? first_bin(k) == digit : k >> shift == prefix))
                     sm.mine[atomicAdd(&sm.n_mine, 1)] = (static_cast<uint64_t>(k) << 32) | static_cast<uint32_t>(~s);
             });
             cluster_sync<C>();
@@ -339,6 +360,11 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
                     sm.key = static_cast<uint32_t>(k >> 32), sm.slot = static_cast<int>(~static_cast<uint32_t>(k));
             }
             found = true;
+        } else if (pass == 0 && (digit == 0 || digit == D::kBins - 1)) {
+            // many outside of the first pass's bins: all over by the leading bits
+            prefix = 0;
+            need = before;
+            shift = 32;
         }
         // the next digit; none is left when the bin is one key
         bits = min(D::kBits, shift);
@@ -439,6 +465,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const CacheEvi
     }
     if (moves_here) {
         cluster_sync<C>();
+        arrive();  // its warp has no moves, or the last ones
         // few: four moves at a time to every 16 lanes of the cluster
         for (int i = (rank * (kThreads / 16) + (tid >> 4)) * 4; i < n; i += C * kThreads / 4)
             move_slots(a, dst, src, at, i, min(n, i + 4));

@@ -490,6 +490,18 @@ def test_evict_shapes(be, rows, kvh, max_len, keep, ties):
     check_evict(be, s, lens, keep, keep // 3, w, p, next_pos, in_place=not ties)
 
 
+@pytest.mark.parametrize("rows,kvh,max_len,keep", [(80, 1, 3000, 1000), (1, 1, 20000, 6000), (3, 2, 2500, 2400)])
+@pytest.mark.parametrize("scale", [1e-24, 1e-13, 1e-7, 1e4, 1e8])
+def test_evict_weights_of_any_size(be, rows, kvh, max_len, keep, scale):
+    """Weights far below and above the usual ones, all different and in few octaves: as many as a histogram can mix."""
+    lens = [max_len - (r * 13) % 40 for r in range(rows)]
+    s = Setup(rows, kvh, max_len, seed=rows)
+    _, p, next_pos = fill_state(s, lens, seed=7, ties=False)
+    w = (scale * (1.0 + np.random.default_rng(rows).random(p.shape))).astype(np.float32)
+    s.w.copy_(cu.torch().from_numpy(w))
+    check_evict(be, s, lens, keep, keep // 5, w, p, next_pos, True)
+
+
 def test_evict_equal_and_special_weights(be):
     """All weights equal (ties by slot), NaN last, infinities and negatives in order, denormals, every slot recent."""
     lens = [200] * 5
