@@ -24,8 +24,8 @@ constexpr int kPlanTile = 64;
 constexpr int kPlanTiered = 32;  // tiles a worker from which on work is taken dynamically
 constexpr int kPlanSmall = 3;    // the least tiles of a tier
 constexpr int kPlanWhole = 2;    // tiles a worker from which on short runs are spared
-constexpr int kPlanSnap = 8;     // runs up to so many tiles are not cut
-constexpr int kPlanReach = 4;    // how far a cut moves to spare a run
+constexpr int kPlanSnap = 6;     // runs up to so many tiles are not cut
+constexpr int kPlanReach = 3;    // how far a cut moves to spare a run
 
 // n / d for 0 <= n < 2^24, d > 0.
 Q3_HD int plan_quotient(int n, int d) {
@@ -71,13 +71,13 @@ Q3_HD int equal_share_of(const Equal& e, int t) {
 // region gives the order of taking; the order along the tiles is region * tiers + tier.
 //
 // A cut inside a run costs a part to write and to join, so from two tiles a worker on
-// cuts move to a run's nearer end where the run has at most 8 tiles, or the end is at
+// cuts move to a run's nearer end where the run has at most 6 tiles, or the end is at
 // most 2 tiles away (plan_down, plan_up).  With less work a run's tiles side by side are
 // worth their parts: 5 tiles in each of 8 runs take 8.7 us apart and 10.3 us together,
 // 64 in each of 8 12.5 and 14.0 us; from four tiles a worker on instead of two, 200
 // sequences of 1 .. 500 slots take 19.5 us for 18.6.  A chunk may be empty then; those of one run are consecutive.
-// Sparing runs of up to 4 tiles alone, 200 sequences of 1 .. 500 slots take 19.9 us for
-// 18.7, and 20 of up to 638 with 8 heads 16.8 for 17.5.
+// Sparing runs of up to 4, 6 and 8 tiles, 200 sequences of 1 .. 500 slots take 18.4, 17.9
+// and 18.1 us, and 20 of up to 638 with 8 heads 16.1, 16.0 and 16.5.
 Q3_HD int plan_rest(int base) { return base / 8 * 3 + base % 8 * 3 / 8; }
 struct Plan {
     Equal region;
