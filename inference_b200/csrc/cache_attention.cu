@@ -95,6 +95,7 @@ struct Parts {
     float* po;     // [chunk's place][2][G][128]: unnormalised outputs of parts
     float* score;  // [tile][64][G]: raw scores in log2 units
     int workers;
+    uint32_t inverse;  // of workers
 };
 
 // 2^x by the exponential unit: off by 2 units of 2^-23 at most, results below 2^-126 are 0.
@@ -126,9 +127,20 @@ __device__ __forceinline__ void scan_rows(const int32_t* lens, const CacheView& 
     __syncthreads();
 }
 
-template <int THREADS>
-__device__ __forceinline__ PlanPlace locate(int t, const int32_t* lens, const CacheView& c, const int* before) {
-    return plan_locate(t, lens, c.rows, c.max_len, c.kv_heads, before, THREADS);
+// The same by one warp, in 32 groups: `per` rows a lane.
+__device__ __forceinline__ void scan_rows_warp(const int32_t* lens, const CacheView& c, int per, int* before) {
+    const int lane = threadIdx.x & 31;
+    int incl = 0;
+#pragma unroll 4
+    for (int r = lane * per; r < min(c.rows, lane * per + per); ++r) incl += plan_tiles(lens[r], c.max_len);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    before[lane + 1] = incl;
+    if (lane == 0) before[0] = 0;
+    __syncwarp();
 }
 
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
@@ -165,14 +177,20 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
         prefetch_map(&maps.k16);
         prefetch_map(&maps.v16);
     }
+    __syncthreads();  // the barriers are set up
     pdl_wait();     // what ran before may have written the lengths, queries and pages
     pdl_trigger();  // the joining kernel may set itself up; it waits for this one's end
-    scan_rows<kThreads>(a.lens, c, sm.before, sm.scan);
+    // only the producer looks tiles up: few rows it scans by itself
+    const bool few = c.rows <= 256;
+    if (!few) scan_rows<kThreads>(a.lens, c, sm.before, sm.scan);
 
     if (warp == kWarps) {
         // ------------------------------------------------------------ producer
-        const int total = sm.before[kThreads] * c.kv_heads;
-        const Plan plan = plan_make(total, parts.workers);
+        const int groups = few ? 32 : kThreads;
+        const int per = few ? (c.rows + 31) / 32 : plan_group_rows(c.rows, kThreads);
+        if (few) scan_rows_warp(a.lens, c, per, sm.before);
+        const int total = sm.before[groups] * c.kv_heads;
+        const Plan plan = plan_make(total, parts.workers, parts.inverse);
         const uint64_t pol = policy_evict_first();
         int k = 0, s = 0, round = 0;  // tiles sent for; the stage for the next, used `round` times before
         bool ok = true;
@@ -192,7 +210,7 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                 bool here = false;
                 if (i0 + lane < stop) {
                     const int t = i0 + lane;
-                    const PlanPlace p = locate<kThreads>(t, a.lens, c, sm.before);
+                    const PlanPlace p = plan_locate(t, a.lens, c.rows, c.max_len, c.kv_heads, sm.before, groups, per);
                     const int run0 = t - p.tile;
                     auto behind = [&](int tile, int cut) { return plan_behind(plan, run0, p.tiles, tile, cut); };
                     here = behind(p.tile, t0) && (t1 == total || !behind(p.tile, t1));
@@ -577,7 +595,7 @@ __global__ void __maxnreg__(64)
     const int G = a.q_heads / c.kv_heads;
     scan_rows<kJoinThreads>(a.lens, c, sm.before, sm.scan);
     const int total = sm.before[kJoinThreads] * c.kv_heads;
-    const Plan plan = plan_make(total, parts.workers);
+    const Plan plan = plan_make(total, parts.workers, parts.inverse);
     const Equal mine = equal_make(total, gridDim.x);
     const int t0 = equal_first(mine, me), t1 = equal_first(mine, me + 1);
     // the runs met by tiles [t, t + 64) of the share
@@ -588,7 +606,8 @@ __global__ void __maxnreg__(64)
         bool starts = false;
         if (tid < kJoinTiles) {
             if (tid < n) {
-                p = locate<kJoinThreads>(t + tid, a.lens, c, sm.before);
+                p = plan_locate(t + tid, a.lens, c.rows, c.max_len, c.kv_heads, sm.before, kJoinThreads,
+                                plan_group_rows(c.rows, kJoinThreads));
                 starts = tid == 0 || p.tile == 0;
             }
             const unsigned who = __ballot_sync(0xffffffffu, starts);
@@ -792,7 +811,7 @@ int workers_of(const CacheView& c, int sms) {
 // The workspace's arrays from its start; returns its size.
 size_t layout(const CacheView& c, int q_heads, int accumulate, int sms, uint8_t* ws, Parts* p) {
     const int G = q_heads / c.kv_heads, workers = workers_of(c, sms);
-    const size_t parts = 2 * static_cast<size_t>(workers) * plan_make(static_cast<int>(max_tiles(c)), workers).tiers;
+    const size_t parts = 2 * static_cast<size_t>(workers) * plan_make(static_cast<int>(max_tiles(c)), workers, plan_inverse(workers)).tiers;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         uint8_t* to = ws + at;
@@ -800,6 +819,7 @@ size_t layout(const CacheView& c, int q_heads, int accumulate, int sms, uint8_t*
         return to;
     };
     p->workers = workers;
+    p->inverse = plan_inverse(workers);
     p->ml = reinterpret_cast<float2*>(take(static_cast<size_t>(c.rows) * q_heads * 8));
     p->pml = reinterpret_cast<float2*>(take(parts * G * 8));
     p->po = reinterpret_cast<float*>(take(parts * G * kCacheHd * 4));

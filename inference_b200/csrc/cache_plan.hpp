@@ -43,6 +43,14 @@ Q3_HD int plan_tiles(int len, int max_len) {
     return len > 0 && len <= max_len ? (len + kPlanTile - 1) / kPlanTile : 0;
 }
 
+// n / d for 0 <= n <= 2^30 from 2^32 / d, rounded up: the product is above the quotient by less than 1 / 4.
+inline uint32_t plan_inverse(int d) { return d > 1 ? static_cast<uint32_t>((1ull << 32) / d + 1) : 0; }
+Q3_HD int plan_over(int n, int d, uint32_t inverse) {
+    if (d == 1) return n;
+    const int q = static_cast<int>((static_cast<uint64_t>(n) * inverse) >> 32);
+    return q - (q * d > n);
+}
+
 // `total` tiles in `parts` equal shares (sizes differ by one): the first tile of share
 // i, and the share that holds tile t.
 struct Equal {
@@ -84,9 +92,10 @@ struct Plan {
     int workers, tiers, chunks;
     int snap, slack;  // runs up to `snap` tiles are not cut; in longer ones cuts move by up to `slack`
 };
-Q3_HD Plan plan_make(int total, int workers) {
+Q3_HD Plan plan_make(int total, int workers, uint32_t inverse) {
     Plan p;
-    p.region = equal_make(total, workers);
+    p.region.base = plan_over(total, workers, inverse);
+    p.region.extra = total - p.region.base * workers;
     p.workers = workers;
     p.tiers = 1;
     p.snap = p.region.base < kPlanWhole ? 0 : kPlanSnap;
@@ -140,8 +149,8 @@ Q3_HD int plan_log2(int n) {
     return 31 - __builtin_clz(n);
 #endif
 }
-// Rows are scanned in `groups` (at most 256) groups of consecutive rows; before[i] = tiles of one
-// head before group i, before[groups] = all.
+// Rows are scanned in `groups` (at most 256) groups of `per` consecutive rows; before[i] = tiles of
+// one head before group i, before[groups] = all.
 Q3_HD int plan_group_rows(int rows, int groups) { return (rows + groups - 1) / groups; }
 
 // Tile t: its row, kv head, index in the run, the run's tiles and the row's length.
@@ -149,13 +158,13 @@ struct PlanPlace {
     int row, head, tile, tiles, len;
 };
 Q3_HD PlanPlace plan_locate(int t, const int32_t* lens, int rows, int max_len, int kv_heads, const int* before,
-                            int groups) {
+                            int groups, int per) {
     // lies in the row that holds tile u of one head
     const int u = (kv_heads & (kv_heads - 1)) == 0 ? t >> plan_log2(kv_heads) : t / kv_heads;
     // the last group that begins at or before u, by steps of 32, 4 and 1 groups whose loads do not wait for
     // one another
     int lo = 0;
-    for (int step = 32; step >= 1; step = step == 32 ? 4 : step == 4 ? 1 : 0) {
+    for (int step = groups > 32 ? 32 : 4; step >= 1; step = step == 32 ? 4 : step == 4 ? 1 : 0) {
         int n = 0;
 #ifdef __CUDA_ARCH__
 #pragma unroll
@@ -165,7 +174,7 @@ Q3_HD PlanPlace plan_locate(int t, const int32_t* lens, int rows, int max_len, i
         lo += n * step;
     }
     PlanPlace p;
-    p.row = lo * plan_group_rows(rows, groups);
+    p.row = lo * per;
     int first = before[lo];
     for (;;) {
         p.len = lens[p.row];

@@ -21,9 +21,10 @@ using namespace q3;
     } while (0)
 
 static void check_totals(int total, int workers) {
-    const Plan p = plan_make(total, workers);
+    const Plan p = plan_make(total, workers, plan_inverse(workers));
+    REQUIRE(p.region.base == total / workers && p.region.extra == total % workers);
     REQUIRE(p.tiers >= 1 && p.tiers <= 31 && p.chunks <= p.tiers * workers);
-    REQUIRE(plan_make(total + 5, workers).tiers >= p.tiers);  // the workspace's bound
+    REQUIRE(plan_make(total + 5, workers, plan_inverse(workers)).tiers >= p.tiers);  // the workspace's bound
     std::vector<std::pair<int, int>> at(static_cast<size_t>(p.tiers) * workers, {-1, -1});
     for (int id = 0; id < p.chunks; ++id) {
         int first = 0, end = 0, place = 0;
@@ -68,7 +69,7 @@ static void check(const std::vector<int32_t>& lens, int kvh, int max_len, int wo
     }
     const int total = static_cast<int>(all.size());
     check_totals(total, workers);
-    const Plan plan = plan_make(total, workers);
+    const Plan plan = plan_make(total, workers, plan_inverse(workers));
     std::vector<int> before(groups + 1, 0);
     const int per = plan_group_rows(rows, groups);
     for (int i = 0; i < groups; ++i) {
@@ -92,7 +93,7 @@ static void check(const std::vector<int32_t>& lens, int kvh, int max_len, int wo
         int t0 = 0, t1 = 0, place = 0;
         plan_chunk(plan, o.second, t0, t1, place);
         for (int t = t0 - kPlanReach < 0 ? 0 : t0 - kPlanReach; t < total && t < t1 + kPlanReach; ++t) {
-            const PlanPlace p = plan_locate(t, lens.data(), rows, max_len, kvh, before.data(), groups);
+            const PlanPlace p = plan_locate(t, lens.data(), rows, max_len, kvh, before.data(), groups, per);
             const T& w = all[t];
             REQUIRE(p.row == w.row && p.head == w.head && p.tile == w.tile && p.tiles == w.tiles &&
                     p.len == lens[w.row]);
@@ -126,7 +127,7 @@ int main() {
             const int kind = pick(0, 9);
             n = kind == 0 ? 0 : kind == 1 ? -pick(1, 100) : kind == 2 ? max_len + pick(1, 9) : pick(0, max_len);
         }
-        check(lens, pick(1, 9), max_len, pick(1, 300), pick(0, 1) ? 160 : 128);
+        check(lens, pick(1, 9), max_len, pick(1, 300), std::vector<int>{32, 128, 160}[pick(0, 2)]);
     }
     check({20000, 3, 500, 9000, 512, 513, 20000}, 3, 20000, 20, 160);
     check(std::vector<int32_t>(4096, 1), 1, 1, 296, 160);
