@@ -159,11 +159,11 @@ class B200Backend:
 
     def _heads(self, name: str, t, n: int, heads: int, index: int) -> int:
         """The row stride of t, a bf16 [n, heads, 128] tensor on device `index` whose rows are contiguous."""
-        shape, stride = t.shape, t.stride()
-        if (t.dtype is not self._bf16 or len(shape) != 3 or shape[0] != n or shape[1] != heads or shape[2] != 128
-                or stride[2] != 1 or (stride[1] != 128 and heads > 1) or t.get_device() != index):
-            raise ValueError(f"{name} must be a bf16 [{n}, {heads}, 128] tensor on {self.device} with contiguous rows")
-        return stride[0] if n > 1 else 128 * heads
+        if t.dtype is self._bf16 and t.shape == (n, heads, 128) and t.get_device() == index:
+            row, head, dim = t.stride()
+            if dim == 1 and (head == 128 or heads == 1):
+                return row if n > 1 else 128 * heads
+        raise ValueError(f"{name} must be a bf16 [{n}, {heads}, 128] tensor on {self.device} with contiguous rows")
 
     def _ints(self, name: str, t, n: int, index: int) -> int:
         if t.dtype is not self._i32 or t.dim() != 1 or t.numel() != n or t.get_device() != index or not t.is_contiguous():
