@@ -28,14 +28,14 @@
 //
 // Measured (B200, captured into a graph, weights accumulated; the share is that of
 // the bytes above at the measured copy rate of 6.55 TB/s):
-//   64 sequences x 8192 slots, 16 / 4 heads   204 us, 94 %  (the score stores are 8 us
+//   64 sequences x 8192 slots, 16 / 4 heads   203 us, 94 %  (the score stores are 8 us
 //                                             of it; the first kernel reads 1.24 GB for
 //                                             1.21 GB of K and V)
-//   one of 100001 slots, 32 / 8 heads          75 us, 83 %
-//   16 of up to 4096, 32 / 8 heads             36 us, 66 %  (join 8 us)
-//   200 of 1 .. 500, 4 / 1 heads               19 us, 25 %  (a worker's longest uncut run
+//   one of 100001 slots, 32 / 8 heads          74 us, 85 %
+//   16 of up to 4096, 32 / 8 heads             35 us, 69 %  (join 7 us)
+//   200 of 1 .. 500, 4 / 1 heads               17.4 us, 26 % (a worker's longest uncut run
 //                                             at 1 us a tile, start, join)
-//   one of 4095 14 us and one of 300 10 us    start, look-ups, one tile's latency, join
+//   one of 4095 10.8 us, one of 300 7.5 us    start, look-ups, one tile's latency, join
 // One kernel with a grid barrier in place of the second launch cost 2.3 us where the
 // programmatic launch costs 0.7; letting the last part of a run find its maximum and sum
 // (a fence and an atomic a part) took 50 us instead of 43 at 16 x 4096.

@@ -75,17 +75,18 @@ Q3_HD int equal_share_of(const Equal& e, int t) {
 // 204 us), and what a worker finishes late is at most a small chunk.  Regions below
 // 32 tiles stay whole: more cuts cost more than they gain.  With tiers and without, 64 x
 // 8192 slots (125 tiles a worker) take 205 and 217 us, one of 100001 (43 tiles) 75 and
-// 73; with tiers from 12 tiles on 16 x 4096 (16 tiles) takes 37.9 us for 36.3.  Chunk id = tier * workers +
-// region gives the order of taking; the order along the tiles is region * tiers + tier.
+// 73; with tiers from 12 tiles on 16 x 4096 (16 tiles) takes 37.9 us for 36.3.  Chunk id =
+// tier * workers + region gives the order of taking; the order along the tiles is region *
+// tiers + tier.
 //
 // A cut inside a run costs a part to write and to join, so from two tiles a worker on
 // cuts move to a run's nearer end where the run has at most 6 tiles, or the end is at
-// most 2 tiles away (plan_down, plan_up).  With less work a run's tiles side by side are
-// worth their parts: 5 tiles in each of 8 runs take 8.7 us apart and 10.3 us together,
-// 64 in each of 8 12.5 and 14.0 us; from four tiles a worker on instead of two, 200
-// sequences of 1 .. 500 slots take 19.5 us for 18.6.  A chunk may be empty then; those of one run are consecutive.
-// Sparing runs of up to 4, 6 and 8 tiles, 200 sequences of 1 .. 500 slots take 18.4, 17.9
-// and 18.1 us, and 20 of up to 638 with 8 heads 16.1, 16.0 and 16.5.
+// most 2 tiles away (plan_down, plan_up).  A chunk may be empty then; those of one run
+// are consecutive.  With less work a run's tiles side by side are worth their parts: 5
+// tiles in each of 8 runs take 8.7 us apart and 10.3 us together, 64 in each of 8 12.5
+// and 14.0 us; from four tiles a worker on instead of two, 200 sequences of 1 .. 500
+// slots take 19.5 us for 18.6.  Sparing runs of up to 4, 6 and 8 tiles, those take 18.4,
+// 17.9 and 18.1 us, and 20 of up to 638 with 8 heads 16.1, 16.0 and 16.5.
 Q3_HD int plan_rest(int base) { return base / 8 * 3 + base % 8 * 3 / 8; }
 struct Plan {
     Equal region;

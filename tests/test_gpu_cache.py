@@ -78,6 +78,18 @@ def test_attention_many_rows(be, accumulate):
         check_attention(be, s, cache, q, lens, accumulate)
 
 
+@pytest.mark.parametrize("rows", [31, 32, 33, 100, 255, 256, 257])
+@pytest.mark.parametrize("most", [40, 400])
+def test_attention_row_counts(be, rows, most):
+    """Row counts around those at which the scan of the lengths changes form, idle rows among them; short and long runs."""
+    rng = np.random.default_rng(rows)
+    lens = [0 if r % 5 == 3 else int(x) for r, x in enumerate(rng.integers(0, most, rows))]
+    s = Setup(rows, 1, most, seed=rows)
+    q = s.randn(rows, 4, HD)
+    with s.cache() as cache:
+        check_attention(be, s, cache, q, lens)
+
+
 def test_attention_most_rows(be):
     """The largest number of sequences, most of them idle."""
     lens = [0] * 4096
