@@ -73,11 +73,12 @@ Q3_HD int equal_share_of(const Equal& e, int t) {
 // are taken by whichever worker is free, the larger ones of all regions first: SMs
 // differ in the bandwidth they get (on a B200, whole regions of 125 tiles took 157 to
 // 204 us), and what a worker finishes late is at most a small chunk.  Regions below
-// 32 tiles stay whole: more cuts cost more than they gain.  With tiers and without, 64 x
-// 8192 slots (125 tiles a worker) take 205 and 217 us, one of 100001 (43 tiles) 75 and
-// 73; with tiers from 12 tiles on 16 x 4096 (16 tiles) takes 37.9 us for 36.3.  Chunk id =
-// tier * workers + region gives the order of taking; the order along the tiles is region *
-// tiers + tier.
+// 32 tiles stay whole: more cuts cost what they gain.  With tiers and without, 64 x 8192
+// slots (125 tiles a worker) take 205 and 217 us, one of 100001 (43 tiles) 75 and 73; 16 x
+// 4096 (15 tiles) takes 34.7 us either way.  Halving down to 5 tiles instead of 3, one of
+// 100001 takes 72.8 us for 74.3 and 73 x 2713 with 8 heads (49 tiles) 80.6 for 79.2.
+// Chunk id = tier * workers + region gives the order of taking; the order along the tiles
+// is region * tiers + tier.
 //
 // A cut inside a run costs a part to write and to join, so from two tiles a worker on
 // cuts move to a run's nearer end where the run has at most 6 tiles, or the end is at
