@@ -492,7 +492,7 @@ typedef struct q3_cache_desc {
     size_t slot_stride;     /* >= max_len */
     size_t rows;            /* sequences, 1 .. 4096 */
     size_t max_len;         /* slots a sequence may hold, 1 .. 2^20 */
-    size_t kv_heads;
+    size_t kv_heads;        /* rows * kv_heads * ceil(max_len / 64) is at most 2^30 */
     size_t head_dim;  /* 128 */
     size_t page_size; /* 64 */
     uint32_t* state_dev; /* Q3_CACHE_STATE_WORDS words, 0 at first and the library's from then on:

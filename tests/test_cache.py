@@ -34,10 +34,20 @@ def cache():
     (dict(kv_heads=0), 1), (dict(rows=0), 1), (dict(rows=4097), 1), (dict(max_len=0), 1),
     (dict(max_len=(1 << 20) + 1), 1), (dict(max_len=129), 1), (dict(slot_stride=127), 1), (dict(num_pages=0), 1),
     (dict(num_pages=1 << 25), 1), (dict(kv_heads=1 << 20), 1),
-    (dict(rows=4096, kv_heads=1024, max_len=1 << 20, table_stride=1 << 14, slot_stride=1 << 20), 1)])
+    (dict(rows=4096, kv_heads=1024, max_len=1 << 20, table_stride=1 << 14, slot_stride=1 << 20), 1),
+    (dict(rows=4096, kv_heads=17, max_len=1 << 20, table_stride=1 << 14, slot_stride=1 << 20), 1)])
 def test_create_refuses(change, status):
     got, h = create(**change)
     assert got == status and not h.value
+
+
+def test_the_largest_cache():
+    from inference_b200 import lib
+
+    status, h = create(rows=4096, kv_heads=16, max_len=1 << 20, table_stride=1 << 14, slot_stride=1 << 20)
+    assert status == 0
+    assert lib().q3_cache_attention_workspace_bytes(h, 256, 1) > 2 ** 30 * 64 * 16 * 4  # the scores alone
+    assert lib().q3_cache_destroy(h) == 0
 
 
 def test_create_without_weights():
