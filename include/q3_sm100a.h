@@ -531,7 +531,11 @@ Q3_API int q3_cache_append(q3_cache* c, const uint16_t* q_dev, size_t q_stride, 
  * kv = qh / (q_heads / kv_heads), fp32 softmax, BF16 out.  q_heads is kv_heads
  * times 1 .. 16.  With accumulate != 0 every slot's softmax probabilities,
  * summed over the query heads of its kv head, are added to its weight.  A
- * sequence of length 0 gets zeros and keeps its weights.  out may be q (with
+ * sequence of length 0 gets zeros and keeps its weights.  An infinite value in a
+ * slot below the length makes its dimension infinite, or NaN where the formula
+ * does; a probability below 2^-126 counts as 0.  Values are summed before the
+ * division by the probabilities' sum (at most the length): that sum must stay
+ * below 2^128.  out may be q (with
  * its stride).  Strides in elements, multiples of 8.  The workspace (16-byte
  * aligned, q3_cache_attention_workspace_bytes) belongs to the call until it has
  * finished on the GPU; unordered calls on different caches need one each. */

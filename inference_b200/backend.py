@@ -211,7 +211,8 @@ class B200Backend:
     def cache_attention(self, cache, query, lens, output, accumulate: bool = True):
         """output[r] = attention of query[r] (bf16 [rows, q_heads, 128], rows may be strided) over slots
         0 .. lens[r] - 1 of sequence r (q3_cache_attention); accumulate adds each slot's probabilities, summed over
-        the query heads of its kv head, to cache.weights.  output may be query."""
+        the query heads of its kv head, to cache.weights.  output may be query.  An infinite value in a slot below the
+        length makes its dimension infinite, or NaN where the formula does."""
         L, index, stream = self._cache_call(cache)
         rows, qh = cache.rows, query.shape[1]
         qs = self._heads("query", query, rows, qh, index)

@@ -105,6 +105,14 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Two BF16 values, infinities and NaN replaced by the largest finite value (with the sign
+// that they have).
+__device__ __forceinline__ uint32_t clamp_bf2(uint32_t x) {
+    uint32_t y;
+    asm("min.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x7F7F7F7Fu));
+    return y;
+}
+
 // Groups of consecutive rows, one per thread: before[t] = tiles (of one kv head)
 // before thread t's rows, before[threads] = all.
 template <int THREADS>
@@ -413,7 +421,9 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                 pl[nt][0] = movmatrix_trans(pack_bf2(lo[0], lo[1]));
                 pl[nt][1] = movmatrix_trans(pack_bf2(lo[2], lo[3]));
             }
-            // ---- O^T += V^T P^T
+            // ---- O^T += V^T P^T.  P's first part is positive where P is, so an infinite value and
+            // NaN come through its product as the formula has them; its second part is of either
+            // sign or 0 and would make NaN of infinity: that product takes finite values alone.
             {
                 const int q = lane >> 3, row = warp * 16 + (q >> 1) * 8 + (lane & 7);
 #pragma unroll
@@ -421,10 +431,10 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
                     uint32_t a0, a1, a2, a3;
                     ldmatrix_x4_trans(vt + tile_off(row, 2 * dt + (q & 1)), a0, a1, a2, a3);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma_bf16_16816(o[nt][dt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-                        mma_bf16_16816(o[nt][dt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
-                    }
+                    for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][dt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+                    a0 = clamp_bf2(a0), a1 = clamp_bf2(a1), a2 = clamp_bf2(a2), a3 = clamp_bf2(a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][dt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
                 }
             }
             if (a.accumulate) {
@@ -724,7 +734,7 @@ __global__ void __maxnreg__(64)
                     const int unit = u + column, h = min(unit, u1 - 1) / (kCacheHd / 4);
                     const float2 ml = sm.ml[r][h];
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    // four parts' loads under way together; behind the last one: that one again, with factor 0
+                    // four parts' loads under way together; behind the last one: that one again, for nothing
                     for (int s0 = c0 + turn; s0 <= c1; s0 += 4 * turns) {
                         float m[4];
                         float4 v[4];
@@ -737,7 +747,8 @@ __global__ void __maxnreg__(64)
                         }
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float f = s0 + i * turns <= c1 ? ex2(m[i] - ml.x) : 0.f;
+                            if (s0 + i * turns > c1) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            const float f = ex2(m[i] - ml.x);
                             x.x += v[i].x * f, x.y += v[i].y * f, x.z += v[i].z * f, x.w += v[i].w * f;
                         }
                     }

@@ -160,6 +160,45 @@ def test_attention_of_nan_and_infinity_in_live_slots(be):
     assert float(s.w[3, 1, 20]) == float(before[3, 1, 20])
 
 
+def infinite_values(s, lens):
+    """Infinite values in live slots, in dimensions of their own: one of either sign in a sequence's first, middle and last
+    slot; both signs in one dimension (NaN by the formula); NaN beside infinity."""
+    tables = s.tables.tolist()
+    for r, n in enumerate(lens):
+        for h in range(s.kvh):
+            for dim, marks in ((3, [(0, math.inf)]), (64, [(n // 2, -math.inf)]), (127, [(n - 1, math.inf)]),
+                               (50, [(0, math.inf), (n - 1, -math.inf)]), (51, [(0, math.nan), (n // 2, math.inf)]),
+                               (52, [(j, math.inf) for j in range(0, n, 50)])):
+                if len(marks) == 1 or n > 1:
+                    for j, value in marks:
+                        s.v[tables[r][j // PAGE], h, j % PAGE, dim] = value
+
+
+@pytest.mark.parametrize("qh,kvh", [(4, 2), (3, 1), (32, 4), (16, 1)])
+@pytest.mark.parametrize("lens", [[1, 64, 70, 16], [2000, 130], [400] * 150, [20000, 3]], ids=lambda v: f"{len(v)}x{v[0]}")
+@pytest.mark.parametrize("even", [True, False])
+def test_attention_of_infinite_values(be, qh, kvh, lens, even):
+    """An infinite value in a live slot makes its dimension infinite, as in the formula: whole runs and cut ones, joined from
+    few parts and many, with probabilities that are exact in BF16 (all scores equal) and that are not."""
+    import torch
+
+    s = Setup(len(lens), kvh, max(lens), seed=qh + len(lens))
+    infinite_values(s, lens)
+    q = torch.zeros(len(lens), qh, HD, dtype=torch.bfloat16, device="cuda") if even else s.randn(len(lens), qh, HD)
+    want, tol, dw, dw_tol = cu.attention(s, q, lens)
+    before, out = s.w.clone(), torch.empty_like(q)
+    with s.cache() as cache:
+        be.cache_attention(cache, q, ints(lens), out)
+        cache.sync()
+    fine, got = torch.isfinite(want), out.double()
+    assert bool(torch.isinf(want).any())
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+    close(got[fine], want[fine], tol[fine], "out")
+    full = before.double() + dw
+    close(s.w, full, dw_tol + full.abs() * 2.0 ** -23, "weights")
+
+
 @pytest.mark.parametrize("bad", ["page_high", "page_negative", "length_high", "length_negative"])
 def test_attention_refuses_bad_device_values(be, bad):
     """A page outside the pool or a length outside the cache poisons its own row (NaN) and no other, leaves that row's
