@@ -115,8 +115,8 @@ __device__ __forceinline__ uint32_t clamp_bf2(uint32_t x) {
 
 // Groups of consecutive rows, one per thread: before[t] = tiles (of one kv head)
 // before thread t's rows, before[threads] = all.
-template <int THREADS>
-__device__ __forceinline__ void scan_rows(const int32_t* lens, const CacheView& c, int* before, int* scan) {
+template <int THREADS, class Lens>
+__device__ __forceinline__ void scan_rows(const Lens& lens, const CacheView& c, int* before, int* scan) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int per = plan_group_rows(c.rows, THREADS);
     int sum = 0;
@@ -538,8 +538,14 @@ __global__ void __maxnreg__(NT == 1 ? 128 : 168)
 // the maximum and sum from the run's parts, joins a slice of the run's outputs (as many
 // slices as CTAs that meet the run) and writes the weights of its own slots.  Two CTAs an
 // SM, small enough to be resident beside two of the first kernel: what depends on the
-// lengths alone (the share's runs) is done while that one runs.  The lengths are safe to
-// read before the wait: the first kernel let this one start only behind its own.
+// lengths alone (the share's runs) is done while that one runs.  The lengths are there
+// before the wait: the first kernel lets this one start only behind its own wait for what
+// wrote them.  An SM's first-level cache may still hold older ones, so they are read from
+// L2, where all SMs' writes meet.
+struct LensBehindL1 {
+    const int32_t* at;
+    __device__ __forceinline__ int operator[](int r) const { return __ldcg(at + r); }
+};
 constexpr int kJoinThreads = 128;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr int kJoinTiles = 64;  // tiles whose runs are looked up at a time, a thread each
@@ -603,7 +609,8 @@ __global__ void __maxnreg__(64)
     const CacheView& c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, me = blockIdx.x;
     const int G = a.q_heads / c.kv_heads;
-    scan_rows<kJoinThreads>(a.lens, c, sm.before, sm.scan);
+    const LensBehindL1 lens{a.lens};
+    scan_rows<kJoinThreads>(lens, c, sm.before, sm.scan);
     const int total = sm.before[kJoinThreads] * c.kv_heads;
     const Plan plan = plan_make(total, parts.workers, parts.inverse);
     const Equal mine = equal_make(total, gridDim.x);
@@ -616,7 +623,7 @@ __global__ void __maxnreg__(64)
         bool starts = false;
         if (tid < kJoinTiles) {
             if (tid < n) {
-                p = plan_locate(t + tid, a.lens, c.rows, c.max_len, c.kv_heads, sm.before, kJoinThreads,
+                p = plan_locate(t + tid, lens, c.rows, c.max_len, c.kv_heads, sm.before, kJoinThreads,
                                 plan_group_rows(c.rows, kJoinThreads));
                 starts = tid == 0 || p.tile == 0;
             }

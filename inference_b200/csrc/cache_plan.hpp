@@ -156,11 +156,13 @@ Q3_HD int plan_log2(int n) {
 Q3_HD int plan_group_rows(int rows, int groups) { return (rows + groups - 1) / groups; }
 
 // Tile t: its row, kv head, index in the run, the run's tiles and the row's length.
+// lens[r] is how the lengths are read: an array, or what reads it in a way of its own.
 struct PlanPlace {
     int row, head, tile, tiles, len;
 };
-Q3_HD PlanPlace plan_locate(int t, const int32_t* lens, int rows, int max_len, int kv_heads, const int* before,
-                            int groups, int per) {
+template <class Lens>
+Q3_HD PlanPlace plan_locate(int t, const Lens& lens, int rows, int max_len, int kv_heads, const int* before, int groups,
+                            int per) {
     // lies in the row that holds tile u of one head
     const int u = (kv_heads & (kv_heads - 1)) == 0 ? t >> plan_log2(kv_heads) : t / kv_heads;
     // the last group that begins at or before u, by steps of 32, 4 and 1 groups whose loads do not wait for

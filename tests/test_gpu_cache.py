@@ -699,6 +699,44 @@ def test_captured_step_replays(be):
         del graphs
 
 
+def test_lengths_written_right_before(be):
+    """Lengths that a kernel writes right before each attention, another set every time: the runs of every call are those of
+    its own lengths, one call after the other and as a graph."""
+    import torch
+
+    rng = np.random.default_rng(17)
+    sets = [[int(x) for x in rng.integers(0, 900, 40)] for _ in range(6)]
+    s = Setup(40, 2, 900, seed=18)
+    q = s.randn(40, 8, HD)
+    want = [cu.attention(s, q, lens) for lens in sets]
+    given = torch.stack([ints(lens) for lens in sets])
+    which, lens = torch.zeros(1, dtype=torch.int64, device="cuda"), ints([0] * 40)
+    start, out = s.w.clone(), torch.empty_like(q)
+
+    def step(cache):
+        torch.index_select(given, 0, which, out=lens.view(1, -1))
+        be.cache_attention(cache, q, lens, out)
+
+    with s.cache() as cache:
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                step(cache)
+        torch.cuda.synchronize()
+        for n in range(60):
+            i = n * 5 % 6
+            s.w.copy_(start)
+            which.fill_(i)
+            step(cache) if n % 2 else g.replay()
+            o, tol, dw, dw_tol = want[i]
+            close(out, o, tol, f"out {n}")
+            full = start.double() + dw
+            close(s.w, full, dw_tol + full.abs() * 2.0 ** -23, f"weights {n}")
+        cache.sync()
+        del g
+
+
 def test_calls_behind_copies_in_a_graph(be):
     """Captured behind a copy and a fill, not a kernel: the calls wait for them."""
     import torch
