@@ -496,8 +496,10 @@ typedef struct q3_cache_desc {
     size_t head_dim;  /* 128 */
     size_t page_size; /* 64 */
     uint32_t* state_dev; /* Q3_CACHE_STATE_WORDS words, 0 at first and the library's from then on:
-                          * the first error that a kernel of this cache met, and the attention's
-                          * work counter */
+                          * the first error that a kernel of this cache met, the attention's work
+                          * counter, the eviction's count of arrivals, one not in use.  Kernels
+                          * write them: they live until the last call (and the last replay of a
+                          * graph that captured one) has finished */
 } q3_cache_desc;
 
 /* The handle works on `device`, whichever device is current when it is used.

@@ -175,7 +175,10 @@ class B200Backend:
         index = self.device.index
         if cache.device.index != index or not cache.h:
             raise ValueError(f"the cache is closed or on {cache.device}, this backend on {self.device}")
-        return lib(), index, self._raw_stream(index)
+        stream = self._raw_stream(index)
+        if stream not in cache._streams:
+            cache._used_on(stream)
+        return lib(), index, stream
 
     def cache_append(self, cache, query, key, value, q_norm, k_norm, rope: RopeCache, token_pos, slots, query_out,
                      epsilon: float, lens_out=None, row_seq=None):

@@ -20,7 +20,11 @@ class PagedCache:
     weights and positions may both be None (no accumulation, no eviction).
     max_len, the slots a sequence may hold, defaults to what the page tables and
     weights cover.  The handle keeps the tensors alive.  Calls on one cache are
-    ordered by the caller: one stream, or events."""
+    ordered by the caller: one stream, or events.  A graph that captured calls
+    on a cache writes the cache's own state words when it is replayed: keep the
+    PagedCache until the graph is dropped.  (Without a graph it may be dropped
+    while its last calls run, on any stream; the tensors given to it follow
+    torch's rules for tensors used on several streams.)"""
 
     def __init__(self, k_pages, v_pages, page_tables, weights=None, positions=None, max_len: int | None = None):
         import torch
@@ -66,13 +70,27 @@ class PagedCache:
         self.h = h
         self._empty, self._uint8, self._need = torch.empty, torch.uint8, {}
         # the zeroed state is there before any stream's kernels can reach it
-        torch.cuda.current_stream(dev).synchronize()
+        stream = torch.cuda.current_stream(dev)
+        stream.synchronize()
+        self._streams = {stream.cuda_stream}  # that the allocator knows to use the state
 
     @staticmethod
     def _check_slots(t, like):
         if t.stride(2) != 1 or t.stride(0) != t.shape[1] * t.stride(1) or t.stride() != like.stride():
             raise ValueError("PagedCache: weights and positions must have contiguous slots and evenly spaced heads, "
                              "laid out alike")
+
+    def _used_on(self, stream):
+        """The first call on `stream`, the current one, which is not that of the construction: kernels there write the
+        state words, so the allocator keeps their memory until that stream has passed what it held when this cache was
+        dropped.  A captured call runs when its graph is replayed, on any stream: the cache outlives the graph."""
+        import torch
+
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                return
+        self.state.record_stream(torch.cuda.current_stream(self.device))
+        self._streams.add(stream)
 
     def _scratch(self, call):
         """A workspace for one call, ("attention", q_heads, accumulate) or ("evict", keep), from torch's

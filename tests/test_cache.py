@@ -170,3 +170,23 @@ def test_lengths_are_read_through_the_callers_reader(tmp_path):
     subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-o", exe, src], check=True)
     r = subprocess.run([exe], capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
+
+
+def test_a_cache_learns_of_every_stream_that_uses_it():
+    """The state words belong to the library: a call on a stream that the allocator does not know yet tells it, once a stream."""
+    import torch
+
+    from inference_b200 import B200Backend
+
+    class Cache:
+        device, h, _streams, told = torch.device("cuda", 0), 1, {5}, []
+
+        def _used_on(self, stream):
+            self.told.append(stream)
+            self._streams.add(stream)
+
+    be, cache = B200Backend(0), Cache()
+    for stream in (5, 7, 7, 5, 9):
+        be._raw_stream = lambda index: stream
+        assert be._cache_call(cache)[1:] == (0, stream)
+    assert cache.told == [7, 9]

@@ -847,3 +847,52 @@ def test_calls_on_two_streams(be):
             assert same(outs[i], alone[i][0]) and same(sets[i].w, alone[i][1])
     for c in caches:
         c.close()
+
+
+def test_cache_dropped_behind_a_call_on_another_stream(be):
+    """A cache made on one stream, used on another and dropped while that one is busy: the memory of its state words is not
+    given out again before the other stream is done."""
+    import torch
+
+    s = Setup(3, 2, 100, seed=61)
+    q, lens = s.randn(3, 8, HD), ints([100, 5, 64])
+    want, tol, _, _ = cu.attention(s, q, lens.tolist())
+    side, out = torch.cuda.Stream(), torch.empty_like(q)
+    torch.cuda.synchronize()
+    cache = s.cache()
+    at = cache.state.data_ptr()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)  # some 0.2 s
+        be.cache_attention(cache, q, lens, out)
+    cache.close()
+    del cache
+    others = [torch.zeros(4, dtype=torch.int32, device="cuda") for _ in range(64)]
+    assert not side.query() and at not in [t.data_ptr() for t in others]
+    torch.cuda.synchronize()
+    close(out, want, tol)
+    assert not any(bool(t.any()) for t in others)
+
+
+def test_captured_calls_do_not_mark_streams(be):
+    """Calls on a capturing stream leave the allocator's records alone, and the graph replays."""
+    import torch
+
+    s = Setup(2, 2, 100, seed=62)
+    q, lens, out = s.randn(2, 8, HD), ints([100, 7]), torch.empty(2, 8, HD, dtype=torch.bfloat16, device="cuda")
+    want, tol, _, _ = cu.attention(s, q, lens.tolist())
+    with s.cache() as cache:
+        known = set(cache._streams)
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                be.cache_attention(cache, q, lens, out, accumulate=False)
+        assert cache._streams == known
+        g.replay()
+        torch.cuda.synchronize()
+        close(out, want, tol)
+        with torch.cuda.stream(side):
+            be.cache_attention(cache, q, lens, out, accumulate=False)
+        assert cache._streams == known | {side.cuda_stream}
+        cache.sync()
+        del g
