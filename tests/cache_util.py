@@ -68,8 +68,8 @@ def attention(s: Setup, q, lens):
     (2^-23 each where the adder truncates) of the sum of the products' sizes; that and the scaling
     (2^-23 of the score) give every score an error of at most d.  Numerator and denominator of a probability are each off by
     exp(d) - 1, and by 2^-20 for exp2 (2 units of 2^-23), the sum over slots (a tree of at most 2^-23 a level, and 64 terms
-    in line) and the division.  The output adds 2^-15 of sum p |v| (probabilities carried as two BF16 parts: 2^-16; sums),
-    and its one rounding to BF16, 2^-8."""
+    in line) and the division.  The output adds 2^-15 of sum p |v| (the sums' roundings, 2^-23 each where the adder
+    truncates), and its one rounding to BF16, 2^-8."""
     t = torch()
     rows, qh = q.shape[0], q.shape[1]
     G = qh // s.kvh

@@ -160,6 +160,42 @@ def test_attention_of_nan_and_infinity_in_live_slots(be):
     assert float(s.w[3, 1, 20]) == float(before[3, 1, 20])
 
 
+def test_attention_keeps_the_probabilities_bits(be):
+    """Outputs that cancel down to the last bits of a probability.  Three slots with p = 1, p1 = 2^x of -1 < x < 0 and
+    p2 near 2^-7 (the division by their sum L comes last), values -c0, 1 and -c2 with c0 = p1 rounded to BF16 and
+    c2 = (p1 - c0) / p2 rounded to BF16: what is left is below 2^-17.
+
+    Tolerance: times L, the exponential's 2^-22 of p1 <= 1, the scaling's roundings 2^-24 of |x| < 1 twice, and the sum:
+    three parts' products of three slots, each term cut below 2^-23 of the largest, 1: 9 * 2^-23; together below
+    12 * 2^-23 (1.4e-6; a probability held in 16 bits is off by up to 2^-18, 3.8e-6).  What p2 is off by is multiplied
+    by c2 < 2^-2 and falls inside of it.  Then one rounding to BF16."""
+    import torch
+
+    rows, kvh = 64, 8
+    s = Setup(rows, kvh, 3, seed=71)
+    q = torch.zeros(rows, kvh, HD, dtype=torch.bfloat16, device="cuda")
+    q[:, :, 0] = 1.0
+    s.k.zero_()
+    first = s.tables[:, 0].long()
+    s.k[first, :, 1, 0] = -torch.linspace(0.1, 7.8, rows * kvh, device="cuda").view(rows, kvh).bfloat16()
+    s.k[first, :, 2, 0] = -55.0
+    p = torch.exp(s.k[first, :, :3, 0].double() / HD ** 0.5)  # [rows, kvh, 3]
+    p1, p2 = p[..., 1], p[..., 2]
+    c0 = p1.bfloat16()
+    c2 = ((p1 - c0.double()) / p2).bfloat16()
+    s.v[first, :, 0] = -c0[..., None]
+    s.v[first, :, 1] = 1.0
+    s.v[first, :, 2] = -c2[..., None]
+    total = p.sum(dim=-1)
+    want = (p1 - c0.double() - p2 * c2.double()) / total
+    assert float((want * total).abs().max()) < 2.0 ** -17 and float(c2.double().abs().max()) <= 0.26
+    out = torch.empty_like(q)
+    with s.cache() as cache:
+        be.cache_attention(cache, q, ints([3] * rows), out)
+        cache.sync()
+    close(out, want[..., None].expand_as(out), (12 * 2.0 ** -23 / total + want.abs() * 2.0 ** -8)[..., None].expand_as(out))
+
+
 def infinite_values(s, lens):
     """Infinite values in live slots, in dimensions of their own: one of either sign in a sequence's first, middle and last
     slot; both signs in one dimension (NaN by the formula); NaN beside infinity."""
