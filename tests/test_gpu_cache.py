@@ -269,6 +269,42 @@ def test_attention_refuses_bad_device_values(be, bad):
     assert same(s.w[1], before[1])
 
 
+def test_bad_pages_in_runs_of_one_worker(be):
+    """Enough tiles that runs are finished where they were begun, and long ones that are cut: bad pages in the first, a
+    middle and the last tile of short and long runs.  Their rows become NaN and keep their weights, all others (bad entries
+    behind the length among them) are those of the 64-bit form."""
+    import torch
+
+    from inference_b200 import Q3Error
+
+    rng = np.random.default_rng(73)
+    lens = [int(x) for x in rng.integers(200, 351, 300)]
+    lens[7], lens[100], lens[299] = 2000, 1999, 2000
+    s = Setup(300, 2, 2000, seed=74)
+    q = s.randn(300, 8, HD)
+    want, tol, dw, dw_tol = cu.attention(s, q, lens)
+    before = s.w.clone()
+    pool = s.k.shape[0]
+    for r, page, value in ((0, 0, pool), (3, 1, -1), (4, (lens[4] - 1) // PAGE, 1 << 30), (7, 0, pool), (100, 17, -7),
+                           (299, 31, pool + 3), (298, 0, -1), (298, 1, -1), (50, 2, -1 << 31)):
+        s.tables[r, page] = value
+    bad = [0, 3, 4, 7, 50, 100, 298, 299]
+    s.tables[1, (lens[1] + PAGE - 1) // PAGE:] = -1  # no slot lies there
+    out = torch.zeros_like(q)
+    with s.cache() as cache:
+        for accumulate in (True, False):
+            be.cache_attention(cache, q, ints(lens), out, accumulate=accumulate)
+            with pytest.raises(Q3Error, match="page"):
+                cache.sync()
+            assert bool(torch.isnan(out[bad]).all())
+            good = [r for r in range(300) if r not in bad]
+            close(out[good], want[good], tol[good], "out")
+            full = before.double() + dw
+            close(s.w[good], full[good], (dw_tol + full.abs() * 2.0 ** -23)[good], "weights")
+            assert same(s.w[bad], before[bad])
+            out.zero_()
+
+
 def test_attention_of_a_full_gpu(be):
     """Enough tiles that chunks are taken dynamically, in several tiers, and runs are cut into many parts; twice, for the
     same bits whoever takes what."""
@@ -472,6 +508,45 @@ def test_append_of_many_rows(be, qh, kvh):
     want_v[page, :, at] = v[live]
     want_w[seq, :, slot] = 0.0
     want_p[seq, :, slot] = ints(token_pos)[live][:, None]
+    assert same(s.k, want_k) and same(s.v, want_v) and same(s.w, want_w) and same(s.pos, want_p)
+
+
+@pytest.mark.parametrize("n,qh,kvh", [(600, 64, 8), (1500, 32, 8), (300, 64, 8)])
+def test_append_over_its_inputs(be, n, qh, kvh):
+    """Row i into sequence i, the query over the query slice of the QKV rows, the lengths over the slots, rows left out among
+    them: by the streaming form (600 and 1500 rows), which reads slots and rows ahead of what it writes, and by the other."""
+    import torch
+
+    s = Setup(n, kvh, 150, seed=n + qh)
+    rng = np.random.default_rng(n)
+    slots = rng.integers(0, 150, n).astype(np.int32)
+    slots[rng.integers(0, n, n // 9)] = -1
+    token_pos = [int(x) for x in rng.integers(0, 600, n)]
+    live = torch.from_numpy(slots >= 0).cuda()
+    rope = tables(be)
+    wide = s.randn(n, qh + 2 * kvh, HD)
+    was = wide.clone()
+    q, k, v = wide.split([qh, kvh, kvh], dim=1)
+    qn, kn = s.randn(HD), s.randn(HD)
+    want_k, want_v, want_w, want_p = s.k.clone(), s.v.clone(), s.w.clone(), s.pos.clone()
+    lens = torch.from_numpy(slots).cuda()
+    with s.cache() as cache:
+        be.cache_append(cache, q, k, v, qn, kn, rope, ints(token_pos), lens, q, EPS, lens_out=lens)
+        cache.sync()
+    slot = torch.from_numpy(slots).cuda().long()
+    assert torch.equal(lens.long(), torch.where(live, slot + 1, slot))
+    assert same(wide[:, qh:].contiguous(), was[:, qh:].contiguous())
+    assert same(wide[~live].contiguous(), was[~live].contiguous())
+    pos, seq, slot = ints(token_pos).long(), torch.arange(n, device="cuda")[live], slot[live]
+    zq, tq = cu.turn(was[:, :qh], qn, rope.cosine[pos], rope.sine[pos], EPS)
+    close(q[live], zq[live], tq[live], "query")
+    page, at = s.tables[seq, slot // PAGE].long(), slot % PAGE
+    zk, tk = cu.turn(was[:, qh:qh + kvh], kn, rope.cosine[pos], rope.sine[pos], EPS)
+    close(s.k[page, :, at], zk[live], tk[live], "key")
+    want_k[page, :, at] = s.k[page, :, at]
+    want_v[page, :, at] = was[live, qh + kvh:]
+    want_w[seq, :, slot] = 0.0
+    want_p[seq, :, slot] = pos[live][:, None].int()
     assert same(s.k, want_k) and same(s.v, want_v) and same(s.w, want_w) and same(s.pos, want_p)
 
 
