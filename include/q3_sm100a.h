@@ -517,7 +517,8 @@ Q3_API int q3_cache_sync(q3_cache* c, void* stream);
  * are normalised and rotated as q3_qk_norm_rope does at token_pos[i]; queries go
  * to q_out + i * q_out_stride (q_out may be q with its stride), keys and values
  * to slot slots[i] of sequence row_seq[i] (row_seq NULL: sequence i, n <= rows),
- * whose weights become 0 and positions token_pos[i].  lens_out (may be NULL, may
+ * whose weights become 0 and positions token_pos[i] (a prompt's slots too: their
+ * weights grow by the attention of later tokens alone).  lens_out (may be NULL, may
  * be slots): lens_out[i] = slots[i] + 1.  A row with slots[i] = -1 is skipped.
  * Rows of one call have different (sequence, slot) pairs.  The RoPE tables
  * [max_pos, 64] cover positions 0 .. max_pos - 1. */
@@ -539,8 +540,9 @@ Q3_API int q3_cache_append(q3_cache* c, const uint16_t* q_dev, size_t q_stride, 
  * division by the probabilities' sum (at most the length): that sum must stay
  * below 2^128.  out may be q (with
  * its stride).  Strides in elements, multiples of 8.  The workspace (16-byte
- * aligned, q3_cache_attention_workspace_bytes) belongs to the call until it has
- * finished on the GPU; unordered calls on different caches need one each. */
+ * aligned, q3_cache_attention_workspace_bytes: with accumulate 4 bytes a query
+ * head and slot up to max_len, whatever the lengths) belongs to the call until it
+ * has finished on the GPU; unordered calls on different caches need one each. */
 Q3_API size_t q3_cache_attention_workspace_bytes(const q3_cache* c, size_t q_heads, int accumulate);
 Q3_API int q3_cache_attention(q3_cache* c, const uint16_t* q_dev, size_t q_stride, const int32_t* lens_dev,
                               uint16_t* out_dev, size_t out_stride, size_t q_heads, int accumulate,

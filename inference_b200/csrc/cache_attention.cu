@@ -28,16 +28,17 @@
 // are 2 x 64 x 128 x 8 .. 16 multiply-adds against 32 KB to load, and S, P and O stay in
 // registers from one product to the next; ncu has the tensor pipe far from busy.
 //
-// Measured (B200, captured into a graph, weights accumulated; the share is that of
-// the bytes above at the measured copy rate of 6.55 TB/s):
-//   64 sequences x 8192 slots, 16 / 4 heads   203 us, 94 %  (the score stores are 8 us
-//                                             of it; the first kernel reads 1.24 GB for
-//                                             1.21 GB of K and V)
-//   one of 100001 slots, 32 / 8 heads          74 us, 85 %
-//   16 of up to 4096, 32 / 8 heads             35 us, 69 %  (join 7 us)
-//   200 of 1 .. 500, 4 / 1 heads               17.4 us, 26 % (a worker's longest uncut run
+// Measured (B200, captured into a graph, weights accumulated but for the long one; the
+// share is that of the bytes above at the measured copy rate of 6.55 TB/s):
+//   64 sequences of 1118 .. 8192, 32 / 8 heads  204 us, 94 % (without weights 182 us; K and
+//                                             V are 1.24 GB, and the first kernel reads no
+//                                             more)
+//   one of 100001 slots, 64 / 8 heads          74 us, 84 %
+//   16 of 635 .. 4096, 32 / 8 heads            35 us, 68 %  (join 7 us)
+//   200 of 64 .. 500, 8 / 1 heads              18.1 us, 25 % (a worker's longest uncut run
 //                                             at 1 us a tile, start, join)
-//   one of 4095 10.8 us, one of 300 7.5 us    start, look-ups, one tile's latency, join
+//   one of 4095, 32 / 8 heads                  11.1 us      start, look-ups, one tile's
+//   one of 300, 16 / 8 heads                   7.8 us       latency, join
 // One kernel with a grid barrier in place of the second launch cost 2.3 us where the
 // programmatic launch costs 0.7; letting the last part of a run find its maximum and sum
 // (a fence and an atomic a part) took 50 us instead of 43 at 16 x 4096.
@@ -897,6 +898,7 @@ cudaError_t launch_cache_attention(const CacheAttnArgs& a, const CacheMaps& maps
     // two CTAs an SM are resident beside the first kernel's; with 8 tiles a worker or more the work is worth
     // eight, though the others start (and look up their runs) only when that one ends: 64 x 8192 takes 220,
     // 209, 206, 204 and 210 us with 1, 2, 3, 4 and 6 times the workers, 16 x 4096 37.1, 36.7, 36.4, 36.1 and 40.4
+    // (sequences of up to so many slots, 32 / 8 heads)
     const int join_ctas = max_tiles(c) >= 8 * static_cast<size_t>(parts.workers) ? 4 * parts.workers : parts.workers;
     return launch_after(cache_join_kernel, dim3(join_ctas), kJoinThreads, 0, s, a, parts);
 }

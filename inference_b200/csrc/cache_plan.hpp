@@ -71,12 +71,13 @@ Q3_HD int equal_share_of(const Equal& e, int t) {
 // Every worker (CTA) has an equal region of the tiles.  Its first 5/8 are one chunk,
 // which it begins with; the rest is cut into chunks that halve down to 3 tiles and
 // are taken by whichever worker is free, the larger ones of all regions first: SMs
-// differ in the bandwidth they get (on a B200, whole regions of 125 tiles took 157 to
+// differ in the bandwidth they get (on a B200, whole regions of 128 tiles took 157 to
 // 204 us), and what a worker finishes late is at most a small chunk.  Regions below
-// 32 tiles stay whole: more cuts cost what they gain.  With tiers and without, 64 x 8192
-// slots (125 tiles a worker) take 205 and 217 us, one of 100001 (43 tiles) 75 and 73; 16 x
-// 4096 (15 tiles) takes 34.7 us either way.  Halving down to 5 tiles instead of 3, one of
-// 100001 takes 72.8 us for 74.3 and 73 x 2713 with 8 heads (49 tiles) 80.6 for 79.2.
+// 32 tiles stay whole: more cuts cost what they gain.  With tiers and without, 64 sequences
+// of up to 8192 slots with 8 kv heads (128 tiles a worker) take 205 and 217 us, one of
+// 100001 (42 tiles) 75 and 73; 16 of up to 4096 (16 tiles) take 34.7 us either way.  Halving
+// down to 5 tiles instead of 3, the one of 100001 takes 72.8 us for 74.3 and 73 of up to
+// 2713 (49 tiles) 80.6 for 79.2.
 // Chunk id = tier * workers + region gives the order of taking; the order along the tiles
 // is region * tiers + tier.
 //
@@ -85,9 +86,9 @@ Q3_HD int equal_share_of(const Equal& e, int t) {
 // most 2 tiles away (plan_down, plan_up).  A chunk may be empty then; those of one run
 // are consecutive.  With less work a run's tiles side by side are worth their parts: 5
 // tiles in each of 8 runs take 8.7 us apart and 10.3 us together, 64 in each of 8 12.5
-// and 14.0 us; from four tiles a worker on instead of two, 200 sequences of 1 .. 500
-// slots take 19.5 us for 18.6.  Sparing runs of up to 4, 6 and 8 tiles, those take 18.4,
-// 17.9 and 18.1 us, and 20 of up to 638 with 8 heads 16.1, 16.0 and 16.5.
+// and 14.0 us; from four tiles a worker on instead of two, 200 sequences of 64 .. 500
+// slots with one kv head take 19.5 us for 18.6.  Sparing runs of up to 4, 6 and 8 tiles,
+// those take 18.4, 17.9 and 18.1 us, and 20 of up to 638 with 8 heads 16.1, 16.0 and 16.5.
 Q3_HD int plan_rest(int base) { return base / 8 * 3 + base % 8 * 3 / 8; }
 struct Plan {
     Equal region;
